@@ -324,6 +324,65 @@ int lbrr_op_sync(void* stream);
 int lbrr_op_feed_forward_noalloc(const uint16_t* h16, const uint16_t* w1_16, const float* b1, const uint16_t* w2_16,
                                  const float* b2, const float* resid, float* x, int64_t rows, void* stream);
 
+/* ---------------------------------------------------------------------------
+ * Matrix products in 8-bit floating point.  They have no counterpart in the
+ * reference, whose products are fp16; they give the trunk's products (QKV,
+ * out-projection, feed-forward) a form with half the operand bytes and twice
+ * the tensor rate.
+ *
+ * An 8-bit matrix is two arrays.  `q`: e4m3 codes, rows `ldq` bytes apart.
+ * `scales`: one fp32 scale per block of 128 columns and 1 row (activations) or
+ * 128 rows (weights), stored by column block: the scale of q[r][c] is
+ * scales[(c / 128) * lds + r / block_rows].  It stands for q * scale.  A block's
+ * scale is max|v| / 448 (at least 2^-126) and its codes are v / scale rounded
+ * to nearest even; a block that holds an infinity or a NaN has scale NaN and
+ * NaN codes throughout.  Bytes between the last column and the next row are
+ * neither read nor written; they may hold anything.
+ *
+ * All four are asynchronous on `stream` (NULL: the legacy default stream) of
+ * the current device, on which every pointer must lie; none allocates, except
+ * that the first product on a device allocates its status word (make that call
+ * outside a graph capture; during one it is refused with LBRR_ERR_STATE).
+ * Calls keep nothing between them and use no shared workspace, so any number
+ * may run at once.  Distances between rows (ld*) count elements.  Except where
+ * noted, outputs must not overlap inputs.  rows == 0 / m == 0 is no work.
+ * LBRR_ERR_INVALID is returned before any device work.
+ * ------------------------------------------------------------------------- */
+#define LBRR_DT_F32 0
+#define LBRR_DT_F16 1
+#define LBRR_DT_BF16 2
+
+/* x [rows][cols] -> 8 bits, by blocks of block_rows (1 or 128) x 128. */
+int lbrr_op_quant8(const void* x, int32_t x_type, int64_t ldx, int64_t rows, int64_t cols, int32_t block_rows,
+                   uint8_t* q, int64_t ldq, float* scales, int64_t lds, void* stream);
+
+/* Residual addition, RMSNorm and quantisation in one pass (the norms of
+ * src/main.rs:490-554, :616-703 in front of an 8-bit product):
+ *   y = x + resid;  n = y / max(sqrt(mean(y^2) + eps), 1e-12 / sqrt(cols)) * gamma;  q, scales = n by 1 x 128.
+ * eps = 0 is the trunk's norm, y * sqrt(cols) / max(|y|, 1e-12).  The sum is
+ * formed and normed in fp32 and rounded once to resid_type for y.  resid NULL:
+ * y is x and nothing is stored (y must be NULL); y NULL with resid: the sum is
+ * not stored.  resid_type is x_type or LBRR_DT_F32.  y may be resid or x itself
+ * (same pointer, distance and type).  cols is at most 32768, gamma is fp32, 0 <= eps <= 1. */
+int lbrr_op_add_norm_quant8(const void* x, int32_t x_type, int64_t ldx, const void* resid, int32_t resid_type,
+                            int64_t ldr, const float* gamma, float eps, void* y, int64_t ldy, uint8_t* q, int64_t ldq,
+                            float* scales, int64_t lds, int64_t rows, int64_t cols, void* stream);
+
+/* out[m][n] = A W^T + bias[n] + resid[m][n]: A [m][k] scaled by 1 x 128, W [n][k]
+ * scaled by 128 x 128 (the torch Linear layout), fp32 sums, one rounding to
+ * out_type.  a and w must start on 16-byte boundaries with lda and ldw
+ * multiples of 16; any m, n, k >= 1.  bias (fp32) and resid (out_type) may be
+ * NULL; resid may be out itself (same pointer and distance). */
+int lbrr_op_gemm8(const uint8_t* a, int64_t lda, const float* a_scales, int64_t ldas, const uint8_t* w, int64_t ldw,
+                  const float* w_scales, int64_t ldws, const float* bias, const void* resid, int64_t ldr, void* out,
+                  int32_t out_type, int64_t ldo, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* q, scales = gelu(A W^T + bias) by 1 x 128: FF1 with the erf GELU, written as
+ * the operand of the FF2 product.  bias may be NULL. */
+int lbrr_op_gemm8_gelu_quant8(const uint8_t* a, int64_t lda, const float* a_scales, int64_t ldas, const uint8_t* w,
+                              int64_t ldw, const float* w_scales, int64_t ldws, const float* bias, uint8_t* q,
+                              int64_t ldq, float* scales, int64_t lds, int64_t m, int64_t n, int64_t k, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

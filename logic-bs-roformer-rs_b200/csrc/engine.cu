@@ -1946,7 +1946,7 @@ extern "C" int lbrr_separate_song(lbrr_engine* const* engines, int n, const floa
 }
 
 // ---------------------------------------------------------------------------
-static int* op_status() {
+int* lbrr::op_status(bool peek) {
   static std::mutex mu;
   static std::map<int, int*> per_dev;
   int dev = 0;
@@ -1954,6 +1954,7 @@ static int* op_status() {
   std::lock_guard<std::mutex> lk(mu);
   auto it = per_dev.find(dev);
   if (it != per_dev.end()) return it->second;
+  if (peek) return nullptr;
   int* p = nullptr;
   if (cudaMalloc(&p, 64 * sizeof(int)) != cudaSuccess) return nullptr;
   cudaMemset(p, 0, 64 * sizeof(int));

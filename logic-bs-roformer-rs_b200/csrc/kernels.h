@@ -111,6 +111,60 @@ cudaError_t stft_front(const float* x_interleaved, const float* window, const fl
 cudaError_t istft_back(const float2* c2r, const float* window, const float2* twiddles, const float* inv_env,
                        float* out, int len, int T, int channels, int chunks, cudaStream_t st);
 
+// ---- 8-bit floating point with block scales (quant8.cu, gemm8.cu) ------------
+// q: e4m3 codes [rows][ldq]; scales [column blocks][lds], one per 128 columns
+// and per row (or per 128 rows)
+enum class Elem { F32 = 0, F16 = 1, BF16 = 2 };
+constexpr int kNorm8MaxCols = 32768;
+cudaError_t quant8(const void* x, Elem type, int64_t ldx, int rows, int cols, int block_rows, uint8_t* q, int64_t ldq,
+                   float* scales, int64_t lds, cudaStream_t st);
+struct AddNorm8 {
+  const void* x;
+  Elem x_type;
+  int64_t ldx;
+  const void* resid;  // null: no residual (and no y)
+  Elem resid_type;
+  int64_t ldr;
+  const float* gamma;
+  float eps;
+  void* y;  // resid_type, or null
+  int64_t ldy;
+  uint8_t* q;
+  int64_t ldq;
+  float* scales;
+  int64_t lds;
+  int rows, cols;
+};
+cudaError_t add_norm_quant8(const AddNorm8& a, cudaStream_t st);
+// out = A W^T (block-scaled) + bias + resid, or gelu(A W^T + bias) as 8-bit
+// codes q with scales (then out is null)
+struct Gemm8 {
+  const uint8_t* a;
+  int64_t lda;
+  const float* a_scales;
+  int64_t ldas;
+  const uint8_t* w;
+  int64_t ldw;
+  const float* w_scales;
+  int64_t ldws;
+  const float* bias;  // or null
+  const void* resid;  // out's type, or null
+  int64_t ldr;
+  void* out;
+  Elem out_type;
+  int64_t ldo;
+  uint8_t* q;
+  int64_t ldq;
+  float* scales;
+  int64_t lds;
+  int m, n, k;
+};
+cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st);
+
+// Status word of the per-op entry points on the current device (allocated by
+// the first call there; null if that fails).  peek: null instead of allocating.
+int* op_status(bool peek = false);
+
 // cudaFuncSetAttribute (the dynamic shared-memory opt-in) acts on the current
 // device only.  Runs `setup` once per device (devices 0..63, bit d of `done`)
 // before the first launch there; a failed setup is retried on the next call.

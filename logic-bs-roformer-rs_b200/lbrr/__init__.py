@@ -101,6 +101,12 @@ def lib() -> C.CDLL:
         "lbrr_op_feed_forward": ([vp, vp, vp, vp, vp, vp, vp, i64, vp], C.c_int),
         "lbrr_op_sync": ([vp], C.c_int),
         "lbrr_op_feed_forward_noalloc": ([vp, vp, vp, vp, vp, vp, vp, i64, vp], C.c_int),
+        "lbrr_op_quant8": ([vp, i32, i64, i64, i64, i32, vp, i64, vp, i64, vp], C.c_int),
+        "lbrr_op_add_norm_quant8": ([vp, i32, i64, vp, i32, i64, vp, C.c_float, vp, i64, vp, i64, vp, i64, i64, i64,
+                                     vp], C.c_int),
+        "lbrr_op_gemm8": ([vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, i32, i64, i64, i64, i64, vp], C.c_int),
+        "lbrr_op_gemm8_gelu_quant8": ([vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, i64, i64, i64, vp],
+                                      C.c_int),
         "lbrr_f32_to_f16_bits": ([C.c_float], C.c_uint16),
     }
     for name, (args, res) in sig.items():
@@ -119,7 +125,8 @@ HEADER_SYMBOLS = [
     "lbrr_engine_sync", "lbrr_engine_set_option", "lbrr_engine_get_option", "lbrr_engine_wait_probe",
     "lbrr_engine_read_buffer", "lbrr_engine_memory", "lbrr_engine_destroy", "lbrr_separate_song", "lbrr_op_norm_gates",
     "lbrr_op_qkv_rope", "lbrr_op_attention", "lbrr_op_outproj_norm", "lbrr_op_ff1_gelu", "lbrr_op_ff2_resid",
-    "lbrr_op_feed_forward", "lbrr_op_sync", "lbrr_op_feed_forward_noalloc",
+    "lbrr_op_feed_forward", "lbrr_op_sync", "lbrr_op_feed_forward_noalloc", "lbrr_op_quant8",
+    "lbrr_op_add_norm_quant8", "lbrr_op_gemm8", "lbrr_op_gemm8_gelu_quant8",
 ]
 
 
@@ -385,6 +392,157 @@ def feed_forward_noalloc(h16, w1, b1, w2, b2, resid, x, stream=None):
     16 MiB scratch, at most 8192 rows); returns after the work finished."""
     check(lib().lbrr_op_feed_forward_noalloc(_ptr(h16), _ptr(w1), _ptr(b1), _ptr(w2), _ptr(b2), _ptr(resid),
                                              _ptr(x), h16.shape[0], _stream(stream)))
+
+
+# ---------------------------------------------------------------------------
+# Matrix products in 8-bit floating point (include/lbrr_gpu.h): an 8-bit matrix
+# is a torch.float8_e4m3fn tensor q [rows][cols] and a float32 tensor
+# scales [ceil(cols/128)][ceil(rows/block_rows)].
+# ---------------------------------------------------------------------------
+_DT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
+_E4M3 = "torch.float8_e4m3fn"
+
+
+def _bad(what):
+    raise LbrrError(ERR_INVALID, what)
+
+
+def empty8(rows: int, cols: int, block_rows: int = 1, device="cuda"):
+    """Uninitialised (q, scales) for an 8-bit matrix, q's rows padded to start on
+    16-byte boundaries as the products need."""
+    import torch
+    if rows < 0 or cols < 1 or block_rows not in (1, 128):
+        _bad("empty8: needs rows >= 0, cols >= 1 and block_rows 1 or 128")
+    q = torch.empty(rows, cols + -cols % 16, dtype=torch.float8_e4m3fn, device=device)[:, :cols]
+    return q, torch.empty(-(-cols // 128), -(-rows // block_rows), dtype=torch.float32, device=device)
+
+
+def _matrix(t, name, shape, dtypes, like):
+    """Checks a 2-D tensor and returns the distance between its rows (elements)."""
+    if t.dim() != 2 or tuple(t.shape) != shape:
+        _bad(f"{name} must have shape {shape}, has {tuple(t.shape)}")
+    if str(t.dtype) not in dtypes:
+        _bad(f"{name} must be {' or '.join(sorted(dtypes))}, is {t.dtype}")
+    if not t.is_cuda or t.device != like.device:
+        _bad(f"{name} must be on the CUDA device of the first operand ({like.device}), is on {t.device}")
+    rows, cols = shape
+    if cols > 1 and t.stride(1) != 1:
+        _bad(f"{name} must have neighbouring columns next to each other")
+    if rows <= 1:
+        return cols + -cols % 16  # no second row: any distance
+    ld = t.stride(0)
+    if ld < cols:
+        _bad(f"{name} must not have overlapping rows")
+    return ld
+
+
+def _vector(t, name, n, like):
+    if t is None:
+        return
+    if tuple(t.shape) != (n,) or str(t.dtype) != "torch.float32" or (n > 1 and t.stride(0) != 1):
+        _bad(f"{name} must be a contiguous float32 tensor of {n} values")
+    if not t.is_cuda or t.device != like.device:
+        _bad(f"{name} must be on the CUDA device of the first operand ({like.device}), is on {t.device}")
+
+
+def _same_rows(name, t, ld, other_name, other, other_ld):
+    """Refuses an output that overlaps an input other than element for element."""
+    size, osize = t.element_size(), other.element_size()
+    a0, b0 = t.data_ptr(), other.data_ptr()
+    a1 = a0 + size * ((t.shape[0] - 1) * ld + t.shape[1])
+    b1 = b0 + osize * ((other.shape[0] - 1) * other_ld + other.shape[1])
+    if a0 < b1 and b0 < a1 and not (a0 == b0 and ld == other_ld and t.dtype == other.dtype):
+        _bad(f"{name} overlaps {other_name} without being the same tensor")
+
+
+def _call8(like, stream, fn, *args):
+    """Calls an entry point with the operands' device current."""
+    import torch
+    index = like.device.index
+    sdev = getattr(stream, "device_index", None)
+    if sdev is not None and sdev != index:
+        _bad(f"the stream belongs to device {sdev}, the operands to device {index}")
+    if torch.cuda.current_device() == index:
+        check(fn(*args, _stream(stream)))
+    else:
+        with torch.cuda.device(index):
+            check(fn(*args, _stream(stream)))
+
+
+def quant8(x, q, scales, block_rows: int = 1, stream=None):
+    """x [rows][cols] (float32, float16 or bfloat16) -> q, scales by blocks of
+    block_rows (1: activations, 128: weights) x 128."""
+    if x.dim() != 2 or block_rows not in (1, 128):
+        _bad("quant8: needs a matrix x and block_rows 1 or 128")
+    rows, cols = shape = tuple(x.shape)
+    ldx = _matrix(x, "x", shape, _DT, x)
+    ldq = _matrix(q, "q", shape, (_E4M3,), x)
+    lds = _matrix(scales, "scales", (-(-cols // 128), -(-rows // block_rows)), ("torch.float32",), x)
+    _call8(x, stream, lib().lbrr_op_quant8, x.data_ptr(), _DT[str(x.dtype)], ldx, rows, cols, block_rows,
+           q.data_ptr(), ldq, scales.data_ptr(), lds)
+
+
+def add_norm_quant8(x, resid, gamma, y, q, scales, eps: float = 0.0, stream=None):
+    """y = x + resid; RMSNorm(y) * gamma -> q, scales by 1 x 128.  resid (x's dtype
+    or float32) None: the norm of x, y None.  y (resid's dtype) may be resid or x;
+    None: the sum is not stored."""
+    if x.dim() != 2:
+        _bad("add_norm_quant8: x must be a matrix")
+    rows, cols = shape = tuple(x.shape)
+    ldx = _matrix(x, "x", shape, _DT, x)
+    xt = str(x.dtype)
+    rt, ldr, ldy = xt, 0, 0
+    if resid is not None:
+        ldr = _matrix(resid, "resid", shape, (xt, "torch.float32"), x)
+        rt = str(resid.dtype)
+    if y is not None:
+        if resid is None:
+            _bad("y (the sum) needs resid")
+        ldy = _matrix(y, "y", shape, (rt,), x)
+        _same_rows("y", y, ldy, "x", x, ldx)
+        _same_rows("y", y, ldy, "resid", resid, ldr)
+    _vector(gamma, "gamma", cols, x)
+    ldq = _matrix(q, "q", shape, (_E4M3,), x)
+    lds = _matrix(scales, "scales", (-(-cols // 128), rows), ("torch.float32",), x)
+    _call8(x, stream, lib().lbrr_op_add_norm_quant8, x.data_ptr(), _DT[xt], ldx, _ptr(resid), _DT[rt], ldr,
+           _ptr(gamma), eps, _ptr(y), ldy, q.data_ptr(), ldq, scales.data_ptr(), lds, rows, cols)
+
+
+def _product8(a, a_scales, w, w_scales, bias):
+    if a.dim() != 2 or w.dim() != 2:
+        _bad("a and w must be matrices")
+    (m, k), n = a.shape, w.shape[0]
+    f32 = ("torch.float32",)
+    lda = _matrix(a, "a", (m, k), (_E4M3,), a)
+    ldw = _matrix(w, "w", (n, k), (_E4M3,), a)
+    ldas = _matrix(a_scales, "a_scales", (-(-k // 128), m), f32, a)
+    ldws = _matrix(w_scales, "w_scales", (-(-k // 128), -(-n // 128)), f32, a)
+    _vector(bias, "bias", n, a)
+    return m, n, k, (a.data_ptr(), lda, a_scales.data_ptr(), ldas, w.data_ptr(), ldw, w_scales.data_ptr(), ldws,
+                     _ptr(bias))
+
+
+def gemm8(a, a_scales, w, w_scales, out, bias=None, resid=None, stream=None):
+    """out [m][n] = a @ w.T + bias + resid: a [m][k] scaled by 1 x 128, w [n][k] by
+    128 x 128.  out: float32, float16 or bfloat16; resid has its dtype and may be
+    out itself; bias is float32 [n]."""
+    m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
+    ldo = _matrix(out, "out", (m, n), _DT, a)
+    dt, ldr = str(out.dtype), 0
+    if resid is not None:
+        ldr = _matrix(resid, "resid", (m, n), (dt,), a)
+        if m > 0:
+            _same_rows("out", out, ldo, "resid", resid, ldr)
+    _call8(a, stream, lib().lbrr_op_gemm8, *operands, _ptr(resid), ldr, out.data_ptr(), _DT[dt], ldo, m, n, k)
+
+
+def gemm8_gelu_quant8(a, a_scales, w, w_scales, bias, q, scales, stream=None):
+    """q, scales (by 1 x 128) = gelu(a @ w.T + bias): FF1 written as FF2's operand;
+    bias float32 [n] or None."""
+    m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
+    ldq = _matrix(q, "q", (m, n), (_E4M3,), a)
+    lds = _matrix(scales, "scales", (-(-n // 128), m), ("torch.float32",), a)
+    _call8(a, stream, lib().lbrr_op_gemm8_gelu_quant8, *operands, q.data_ptr(), ldq, scales.data_ptr(), lds, m, n, k)
 
 
 def f32_to_f16_bits(v: float) -> int:
