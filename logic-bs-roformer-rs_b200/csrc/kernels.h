@@ -50,7 +50,7 @@ struct RowNorm {
 };
 
 // TMA tensor maps (zero OOB fill).  Defaults: fp16 elements, 128-byte swizzle.
-enum class MapElem { F16, F32 };
+enum class MapElem { F16, F32, BF16, U8 };
 cudaError_t make_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
                         uint32_t box_inner, uint32_t box_outer, MapElem elem = MapElem::F16,
                         CUtensorMapSwizzle swz = CU_TENSOR_MAP_SWIZZLE_128B);

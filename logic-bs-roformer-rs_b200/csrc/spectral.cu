@@ -30,7 +30,12 @@ static EncodeTiledFn encode_fn() {
 }
 
 static CUtensorMapDataType map_dtype(MapElem e) {
-  return e == MapElem::F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  switch (e) {
+    case MapElem::F32: return CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+    case MapElem::BF16: return CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    case MapElem::U8: return CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    default: return CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  }
 }
 
 cudaError_t make_map_2d(CUtensorMap* map, const void* base, uint64_t inner, uint64_t outer, uint64_t row_bytes,
