@@ -130,11 +130,12 @@ struct ScaleStream {
     m = m0 + row;
     nb = n0 / kBlock8 + part;
   }
-  __device__ __forceinline__ float next(const Params8& p, int n_tiles, int row, int part) {
-    if (!more) return 0.0f;
-    float s = 0.0f;
-    if (m < p.g.m && nb * kBlock8 < p.g.n)
-      s = __ldg(p.g.a_scales + kb * p.g.ldas + m) * __ldg(p.g.w_scales + kb * p.g.ldws + nb);
+  // The block's two scales, multiplied where they are used: the loads are not waited for here.
+  __device__ __forceinline__ float2 next(const Params8& p, int n_tiles, int row, int part) {
+    float2 s = make_float2(0.0f, 0.0f);
+    if (!more) return s;
+    if (m < p.g.m) s.x = __ldg(p.g.a_scales + kb * p.g.ldas + m);
+    if (nb * kBlock8 < p.g.n) s.y = __ldg(p.g.w_scales + kb * p.g.ldws + nb);
     if (++kb == p.kb) {
       kb = 0;
       tile += gridDim.x;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kThreads8, 1)
     ss.tile = blockIdx.x;
     ss.kb = 0;
     ss.at_tile(p, n_tiles, row, part);
-    float s0 = ss.next(p, n_tiles, row, part), s1 = ss.next(p, n_tiles, row, part);
+    float2 s0 = ss.next(p, n_tiles, row, part), s1 = ss.next(p, n_tiles, row, part);
     uint32_t c = 0;
     bool ok = true;
     for (int tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
@@ -265,13 +266,14 @@ __global__ void __launch_bounds__(kThreads8, 1)
       for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = 0; kb < p.kb; ++kb, ++c) {
         const int slot = c & 1;
-        const float2 f = make_float2(s0, s0);
+        const float2 cur = s0;
         s0 = s1;
         s1 = ss.next(p, n_tiles, row, part);
         if (!(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status))) break;
         tc_fence_after();
         if (live) {
           const uint32_t t = tm + slot * kN8;
+          const float2 f = make_float2(cur.x * cur.y, cur.x * cur.y);
           uint32_t va[32], vb[32];
           tmem_ld32(t, va);
           tmem_ld_wait(va);

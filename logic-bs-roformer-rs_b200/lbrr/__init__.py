@@ -399,8 +399,19 @@ def feed_forward_noalloc(h16, w1, b1, w2, b2, resid, x, stream=None):
 # is a torch.float8_e4m3fn tensor q [rows][cols] and a float32 tensor
 # scales [ceil(cols/128)][ceil(rows/block_rows)].
 # ---------------------------------------------------------------------------
-_DT = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}
-_E4M3 = "torch.float8_e4m3fn"
+_torch = None
+_DT = {}     # torch dtype -> LBRR_DT_*
+_F32 = _E4M3 = ()
+
+
+def _need_torch():
+    global _torch, _F32, _E4M3
+    if _torch is None:
+        import torch
+        _DT.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _F32, _E4M3 = (torch.float32,), (torch.float8_e4m3fn,)
+        _torch = torch
+    return _torch
 
 
 def _bad(what):
@@ -410,139 +421,158 @@ def _bad(what):
 def empty8(rows: int, cols: int, block_rows: int = 1, device="cuda"):
     """Uninitialised (q, scales) for an 8-bit matrix, q's rows padded to start on
     16-byte boundaries as the products need."""
-    import torch
+    torch = _need_torch()
     if rows < 0 or cols < 1 or block_rows not in (1, 128):
         _bad("empty8: needs rows >= 0, cols >= 1 and block_rows 1 or 128")
     q = torch.empty(rows, cols + -cols % 16, dtype=torch.float8_e4m3fn, device=device)[:, :cols]
     return q, torch.empty(-(-cols // 128), -(-rows // block_rows), dtype=torch.float32, device=device)
 
 
-def _matrix(t, name, shape, dtypes, like):
+def _device8(t, name):
+    dev = t.get_device()
+    if dev < 0:
+        _bad(f"{name} must be on a CUDA device")
+    return dev
+
+
+def _matrix(t, name, rows, cols, dtypes, dev):
     """Checks a 2-D tensor and returns the distance between its rows (elements)."""
-    if t.dim() != 2 or tuple(t.shape) != shape:
-        _bad(f"{name} must have shape {shape}, has {tuple(t.shape)}")
-    if str(t.dtype) not in dtypes:
-        _bad(f"{name} must be {' or '.join(sorted(dtypes))}, is {t.dtype}")
-    if not t.is_cuda or t.device != like.device:
-        _bad(f"{name} must be on the CUDA device of the first operand ({like.device}), is on {t.device}")
-    rows, cols = shape
-    if cols > 1 and t.stride(1) != 1:
+    if t.shape != (rows, cols):
+        _bad(f"{name} must have shape {(rows, cols)}, has {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        _bad(f"{name} must be {' or '.join(sorted(map(str, dtypes)))}, is {t.dtype}")
+    if t.get_device() != dev:
+        _bad(f"{name} must be on the CUDA device of the first operand ({dev}), is on {t.device}")
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
         _bad(f"{name} must have neighbouring columns next to each other")
     if rows <= 1:
         return cols + -cols % 16  # no second row: any distance
-    ld = t.stride(0)
     if ld < cols:
         _bad(f"{name} must not have overlapping rows")
     return ld
 
 
-def _vector(t, name, n, like):
+def _vector(t, name, n, dev):
+    """Address of a contiguous float32 vector on the device, None for None."""
     if t is None:
-        return
-    if tuple(t.shape) != (n,) or str(t.dtype) != "torch.float32" or (n > 1 and t.stride(0) != 1):
+        return None
+    if t.shape != (n,) or t.dtype not in _F32 or (n > 1 and t.stride(0) != 1):
         _bad(f"{name} must be a contiguous float32 tensor of {n} values")
-    if not t.is_cuda or t.device != like.device:
-        _bad(f"{name} must be on the CUDA device of the first operand ({like.device}), is on {t.device}")
+    if t.get_device() != dev:
+        _bad(f"{name} must be on the CUDA device of the first operand ({dev}), is on {t.device}")
+    return t.data_ptr()
 
 
 def _same_rows(name, t, ld, other_name, other, other_ld):
     """Refuses an output that overlaps an input other than element for element."""
-    size, osize = t.element_size(), other.element_size()
     a0, b0 = t.data_ptr(), other.data_ptr()
-    a1 = a0 + size * ((t.shape[0] - 1) * ld + t.shape[1])
-    b1 = b0 + osize * ((other.shape[0] - 1) * other_ld + other.shape[1])
-    if a0 < b1 and b0 < a1 and not (a0 == b0 and ld == other_ld and t.dtype == other.dtype):
+    if a0 == b0 and ld == other_ld and t.dtype == other.dtype:
+        return
+    rows, cols = t.shape
+    if a0 < b0 + other.element_size() * ((rows - 1) * other_ld + cols) and \
+            b0 < a0 + t.element_size() * ((rows - 1) * ld + cols):
         _bad(f"{name} overlaps {other_name} without being the same tensor")
 
 
-def _call8(like, stream, fn, *args):
+def _call8(dev, stream, fn, *args):
     """Calls an entry point with the operands' device current."""
-    import torch
-    index = like.device.index
-    sdev = getattr(stream, "device_index", None)
-    if sdev is not None and sdev != index:
-        _bad(f"the stream belongs to device {sdev}, the operands to device {index}")
-    if torch.cuda.current_device() == index:
-        check(fn(*args, _stream(stream)))
+    torch = _torch
+    if stream is not None and getattr(stream, "device_index", dev) != dev:
+        _bad(f"the stream belongs to device {stream.device_index}, the operands to device {dev}")
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _stream(stream))
     else:
-        with torch.cuda.device(index):
-            check(fn(*args, _stream(stream)))
+        with torch.cuda.device(dev):
+            rc = fn(*args, _stream(stream))
+    if rc != OK:
+        check(rc)
 
 
 def quant8(x, q, scales, block_rows: int = 1, stream=None):
     """x [rows][cols] (float32, float16 or bfloat16) -> q, scales by blocks of
     block_rows (1: activations, 128: weights) x 128."""
+    _need_torch()
     if x.dim() != 2 or block_rows not in (1, 128):
         _bad("quant8: needs a matrix x and block_rows 1 or 128")
-    rows, cols = shape = tuple(x.shape)
-    ldx = _matrix(x, "x", shape, _DT, x)
-    ldq = _matrix(q, "q", shape, (_E4M3,), x)
-    lds = _matrix(scales, "scales", (-(-cols // 128), -(-rows // block_rows)), ("torch.float32",), x)
-    _call8(x, stream, lib().lbrr_op_quant8, x.data_ptr(), _DT[str(x.dtype)], ldx, rows, cols, block_rows,
-           q.data_ptr(), ldq, scales.data_ptr(), lds)
+    rows, cols = x.shape
+    dev = _device8(x, "x")
+    ldx = _matrix(x, "x", rows, cols, _DT, dev)
+    ldq = _matrix(q, "q", rows, cols, _E4M3, dev)
+    lds = _matrix(scales, "scales", -(-cols // 128), -(-rows // block_rows), _F32, dev)
+    _call8(dev, stream, lib().lbrr_op_quant8, x.data_ptr(), _DT[x.dtype], ldx, rows, cols, block_rows, q.data_ptr(),
+           ldq, scales.data_ptr(), lds)
 
 
 def add_norm_quant8(x, resid, gamma, y, q, scales, eps: float = 0.0, stream=None):
     """y = x + resid; RMSNorm(y) * gamma -> q, scales by 1 x 128.  resid (x's dtype
     or float32) None: the norm of x, y None.  y (resid's dtype) may be resid or x;
     None: the sum is not stored."""
+    _need_torch()
     if x.dim() != 2:
         _bad("add_norm_quant8: x must be a matrix")
-    rows, cols = shape = tuple(x.shape)
-    ldx = _matrix(x, "x", shape, _DT, x)
-    xt = str(x.dtype)
-    rt, ldr, ldy = xt, 0, 0
+    rows, cols = x.shape
+    dev = _device8(x, "x")
+    ldx = _matrix(x, "x", rows, cols, _DT, dev)
+    xt = rt = x.dtype
+    presid, ldr, py, ldy = None, 0, None, 0
     if resid is not None:
-        ldr = _matrix(resid, "resid", shape, (xt, "torch.float32"), x)
-        rt = str(resid.dtype)
+        rt = resid.dtype
+        ldr = _matrix(resid, "resid", rows, cols, (xt,) + _F32, dev)
+        presid = resid.data_ptr()
     if y is not None:
         if resid is None:
             _bad("y (the sum) needs resid")
-        ldy = _matrix(y, "y", shape, (rt,), x)
+        ldy = _matrix(y, "y", rows, cols, (rt,), dev)
+        py = y.data_ptr()
         _same_rows("y", y, ldy, "x", x, ldx)
         _same_rows("y", y, ldy, "resid", resid, ldr)
-    _vector(gamma, "gamma", cols, x)
-    ldq = _matrix(q, "q", shape, (_E4M3,), x)
-    lds = _matrix(scales, "scales", (-(-cols // 128), rows), ("torch.float32",), x)
-    _call8(x, stream, lib().lbrr_op_add_norm_quant8, x.data_ptr(), _DT[xt], ldx, _ptr(resid), _DT[rt], ldr,
-           _ptr(gamma), eps, _ptr(y), ldy, q.data_ptr(), ldq, scales.data_ptr(), lds, rows, cols)
+    pgamma = _vector(gamma, "gamma", cols, dev)
+    ldq = _matrix(q, "q", rows, cols, _E4M3, dev)
+    lds = _matrix(scales, "scales", -(-cols // 128), rows, _F32, dev)
+    _call8(dev, stream, lib().lbrr_op_add_norm_quant8, x.data_ptr(), _DT[xt], ldx, presid, _DT[rt], ldr, pgamma, eps,
+           py, ldy, q.data_ptr(), ldq, scales.data_ptr(), lds, rows, cols)
 
 
 def _product8(a, a_scales, w, w_scales, bias):
+    _need_torch()
     if a.dim() != 2 or w.dim() != 2:
         _bad("a and w must be matrices")
-    (m, k), n = a.shape, w.shape[0]
-    f32 = ("torch.float32",)
-    lda = _matrix(a, "a", (m, k), (_E4M3,), a)
-    ldw = _matrix(w, "w", (n, k), (_E4M3,), a)
-    ldas = _matrix(a_scales, "a_scales", (-(-k // 128), m), f32, a)
-    ldws = _matrix(w_scales, "w_scales", (-(-k // 128), -(-n // 128)), f32, a)
-    _vector(bias, "bias", n, a)
-    return m, n, k, (a.data_ptr(), lda, a_scales.data_ptr(), ldas, w.data_ptr(), ldw, w_scales.data_ptr(), ldws,
-                     _ptr(bias))
+    m, k = a.shape
+    n = w.shape[0]
+    dev = _device8(a, "a")
+    kb = -(-k // 128)
+    lda = _matrix(a, "a", m, k, _E4M3, dev)
+    ldw = _matrix(w, "w", n, k, _E4M3, dev)
+    ldas = _matrix(a_scales, "a_scales", kb, m, _F32, dev)
+    ldws = _matrix(w_scales, "w_scales", kb, -(-n // 128), _F32, dev)
+    return dev, m, n, k, (a.data_ptr(), lda, a_scales.data_ptr(), ldas, w.data_ptr(), ldw, w_scales.data_ptr(), ldws,
+                          _vector(bias, "bias", n, dev))
 
 
 def gemm8(a, a_scales, w, w_scales, out, bias=None, resid=None, stream=None):
     """out [m][n] = a @ w.T + bias + resid: a [m][k] scaled by 1 x 128, w [n][k] by
     128 x 128.  out: float32, float16 or bfloat16; resid has its dtype and may be
     out itself; bias is float32 [n]."""
-    m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
-    ldo = _matrix(out, "out", (m, n), _DT, a)
-    dt, ldr = str(out.dtype), 0
+    dev, m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
+    ldo = _matrix(out, "out", m, n, _DT, dev)
+    dt = out.dtype
+    presid, ldr = None, 0
     if resid is not None:
-        ldr = _matrix(resid, "resid", (m, n), (dt,), a)
+        ldr = _matrix(resid, "resid", m, n, (dt,), dev)
+        presid = resid.data_ptr()
         if m > 0:
             _same_rows("out", out, ldo, "resid", resid, ldr)
-    _call8(a, stream, lib().lbrr_op_gemm8, *operands, _ptr(resid), ldr, out.data_ptr(), _DT[dt], ldo, m, n, k)
+    _call8(dev, stream, lib().lbrr_op_gemm8, *operands, presid, ldr, out.data_ptr(), _DT[dt], ldo, m, n, k)
 
 
 def gemm8_gelu_quant8(a, a_scales, w, w_scales, bias, q, scales, stream=None):
     """q, scales (by 1 x 128) = gelu(a @ w.T + bias): FF1 written as FF2's operand;
     bias float32 [n] or None."""
-    m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
-    ldq = _matrix(q, "q", (m, n), (_E4M3,), a)
-    lds = _matrix(scales, "scales", (-(-n // 128), m), ("torch.float32",), a)
-    _call8(a, stream, lib().lbrr_op_gemm8_gelu_quant8, *operands, q.data_ptr(), ldq, scales.data_ptr(), lds, m, n, k)
+    dev, m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
+    ldq = _matrix(q, "q", m, n, _E4M3, dev)
+    lds = _matrix(scales, "scales", -(-n // 128), m, _F32, dev)
+    _call8(dev, stream, lib().lbrr_op_gemm8_gelu_quant8, *operands, q.data_ptr(), ldq, scales.data_ptr(), lds, m, n, k)
 
 
 def f32_to_f16_bits(v: float) -> int:
