@@ -8,35 +8,46 @@
 // by the tensor core in TMEM, then multiplied once by its two scales and added
 // to the 32-bit total in registers.
 //
-// One persistent CTA per SM walks 128 x 256 tiles.  A K-block of 128 is four
-// tcgen05.mma (kind::f8f6f4, 128 x 256 x 32) into one of two 256-column
-// accumulators, so the tensor core works on block b + 1 while eight warps
-// (two per TMEM lane quadrant, one accumulator row per thread, 128 of the 256
-// columns each) read block b, scale it and add it to 128 totals per thread.
-// A 128-column part is one scale block of W, so the factor of a block is one
-// number per thread.  After the last block the same warps write the tile
-// through shared memory and TMA stores while the tensor core runs ahead into
+// A pair of CTAs (cluster of two, cta_group::2) walks 256 x 256 tiles, each CTA
+// holding 128 rows of A, half of W's rows and the totals of its own 128 rows:
+// against one CTA per 128 x 256 tile the operands' L2 traffic falls by a third,
+// which is what bounded large products (12 TB/s of L2 reads).  A K-block of 128
+// is four tcgen05.mma (kind::f8f6f4, 256 x 256 x 32) into one of two 256-column
+// accumulators, so the tensor cores work on block b + 1 while eight warps of
+// each CTA (two per TMEM lane quadrant, one accumulator row per thread, 128 of
+// the 256 columns each) read block b, scale it and add it to 128 totals per
+// thread.  A 128-column part is one scale block of W, so the factor of a block
+// is one number per thread.  After the last block the same warps write the tile
+// through shared memory and TMA stores while the tensor cores run ahead into
 // the next tile.  Warps: 0..7 totals and output, 8 TMA loads, 9 TMEM
-// allocation and MMA issue, 10 and 11 idle (they complete the warpgroup that
-// gives its registers away).
-#include "gelu.cuh"
+// allocation and (CTA 0) MMA issue, 10 the blocks' scales and 11 the tile's
+// bias (asynchronous copies into rings in shared memory, so the output warps
+// never wait for a global load).
+#include <atomic>
+
+#include "fastdiv.cuh"
+#include "gelu8.cuh"
 #include "quant8.cuh"
 
 namespace lbrr {
 
 constexpr int kM8 = 128, kN8 = 256, kK8 = 128;
-constexpr int kStages8 = 3;
-constexpr int kA8Bytes = kM8 * kK8, kB8Bytes = kN8 * kK8;  // 16 KB, 32 KB
+constexpr int kStages8 = 4;
+constexpr int kA8Bytes = kM8 * kK8, kB8Bytes = kN8 / 2 * kK8;  // 16 KB each: 128 rows of A, half of the tile's W rows
 constexpr int kStage8Bytes = kA8Bytes + kB8Bytes;
 constexpr int kOutWarps8 = 8;
 constexpr int kPart8 = kN8 / 2;                             // columns per output warp
 constexpr int kBuf8Words = 1024;                            // 32 rows x 128 bytes; two per output warp
 constexpr int kBuf8Off = kStages8 * kStage8Bytes;
-constexpr int kBias8Off = kBuf8Off + kOutWarps8 * 2 * kBuf8Words * 4;
-constexpr int kBar8Off = kBias8Off + kOutWarps8 * kPart8 * 4;
-constexpr int kSmem8 = kBar8Off + 256;
+constexpr int kScaleSlots8 = 8;                             // K-blocks
+constexpr int kScaleFloats8 = kM8 + 4;                      // a slot: 128 rows' scales, then W's of the two parts
+constexpr int kScale8Off = kBuf8Off + kOutWarps8 * 2 * kBuf8Words * 4;
+constexpr int kBias8Off = kScale8Off + kScaleSlots8 * kScaleFloats8 * 4;  // two tiles' bias
+constexpr int kBar8Off = kBias8Off + 2 * kN8 * 4;
+constexpr int kSmem8 = kBar8Off + 512;
 constexpr int kThreads8 = kOutWarps8 * 32 + 128;
-constexpr int kLoadWarp8 = kOutWarps8, kMmaWarp8 = kOutWarps8 + 1;
+constexpr int kLoadWarp8 = kOutWarps8, kMmaWarp8 = kOutWarps8 + 1, kScaleWarp8 = kOutWarps8 + 2,
+              kBiasWarp8 = kOutWarps8 + 3;
 constexpr int kRegsOut8 = 216, kRegsOther8 = 72;
 constexpr int kLaunchRegs8 = 168;
 static_assert(kSmem8 <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
@@ -62,7 +73,8 @@ struct OutType<Out8::Q8> {
 
 struct Params8 {
   Gemm8 g;
-  int mt, nt, group;  // row tiles, column tiles, row tiles per group
+  int mt, nt;          // row tiles (of the pair), column tiles
+  FastDiv per;         // division by kGroup8 * nt, the tiles of a group
   int kb;             // K-blocks
   bool out_tma;       // the output's rows allow TMA stores
   bool out_tail;      // ... of a last, partial block too: a TMA store ends on a 16-byte boundary, not on the
@@ -70,20 +82,34 @@ struct Params8 {
   bool resid_vec;     // the residual's rows allow 16-byte loads
 };
 
-// Tiles in groups of `group` row tiles, rows fastest: the CTAs running at one
+// Tiles in groups of kGroup8 row tiles, rows fastest: the pairs running at one
 // time share both their A rows and their W rows in L2.
+constexpr int kGroup8 = 8;
 __device__ __forceinline__ void tile8(const Params8& p, int idx, int& m0, int& n0) {
-  const int per = p.group * p.nt, gi = idx / per, rem = idx - gi * per;
-  const int rows = min(p.group, p.mt - gi * p.group);
-  const int n = rem / rows;
-  m0 = (gi * p.group + rem - n * rows) * kM8;
+  const int gi = p.per.div(idx), rem = idx - gi * (kGroup8 * p.nt);
+  const int rows = p.mt - gi * kGroup8;
+  const int n = rows >= kGroup8 ? rem / kGroup8 : rem / rows;
+  m0 = (gi * kGroup8 + rem - n * min(rows, kGroup8)) * (2 * kM8);
   n0 = n * kN8;
 }
 
 __device__ __forceinline__ void cp_async16(void* dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// 4 bytes, or zero where `valid` is false.
+__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// Arrive on the barrier (one of its counted arrivals) once this thread's copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 
 // Byte o of row r in a buffer of 32 rows of 128 bytes with the TMA 128-byte swizzle.
 __device__ __forceinline__ uint32_t swz(int r, int o) {
@@ -116,50 +142,29 @@ __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t 
       dst[r * ld + c] = *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T))));
 }
 
-__device__ __forceinline__ float4 lds4f(const float* p) { return *reinterpret_cast<const float4*>(p); }
-
-// The scales of the K-blocks to come, two ahead of their use and across tiles.
-struct ScaleStream {
-  int tile, kb, m, nb;
-  bool more;
-  __device__ __forceinline__ void at_tile(const Params8& p, int n_tiles, int row, int part) {
-    more = tile < n_tiles;
-    if (!more) return;
-    int m0, n0;
-    tile8(p, tile, m0, n0);
-    m = m0 + row;
-    nb = n0 / kBlock8 + part;
-  }
-  // The block's two scales, multiplied where they are used: the loads are not waited for here.
-  __device__ __forceinline__ float2 next(const Params8& p, int n_tiles, int row, int part) {
-    float2 s = make_float2(0.0f, 0.0f);
-    if (!more) return s;
-    if (m < p.g.m) s.x = __ldg(p.g.a_scales + kb * p.g.ldas + m);
-    if (nb * kBlock8 < p.g.n) s.y = __ldg(p.g.w_scales + kb * p.g.ldws + nb);
-    if (++kb == p.kb) {
-      kb = 0;
-      tile += gridDim.x;
-      at_tile(p, n_tiles, row, part);
-    }
-    return s;
-  }
-};
+// Columns of the pair's tile that the MMA computes: whole 32s, 16 per CTA's half of W.
+__device__ __forceinline__ int tile_cols8(const Params8& p, int n0) { return min(kN8, (p.g.n - n0 + 31) & ~31); }
 
 template <Out8 O>
-__global__ void __launch_bounds__(kThreads8, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ Params8 p, int* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
   using T = typename OutType<O>::T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBar8Off);
+  const uint32_t rank = cluster_rank();
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBar8Off);  // CTA 0's: both CTAs' loads
   uint64_t* empty = full + kStages8;
   uint64_t* acc_full = empty + kStages8;  // [2]
-  uint64_t* acc_empty = acc_full + 2;     // [2]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  uint64_t* acc_empty = acc_full + 2;     // [2], CTA 0's: both CTAs' output warps
+  uint64_t* sc_full = acc_empty + 2;                // [kScaleSlots8], 32 lanes' copies
+  uint64_t* sc_empty = sc_full + kScaleSlots8;      // [kScaleSlots8]
+  uint64_t* bias_full = sc_empty + kScaleSlots8;    // [2], 32 lanes' copies
+  uint64_t* bias_empty = bias_full + 2;             // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bias_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
-  if ((smem_u32(smem) & 1023u) != 0) {
+  if ((smem_u32(smem) & 1023u) != 0) {  // the same in both CTAs: nothing allocated yet
     if (threadIdx.x == 0) report_status(status, kDevSmemMisaligned);
     return;
   }
@@ -170,7 +175,13 @@ __global__ void __launch_bounds__(kThreads8, 1)
     }
     for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 1);
-      mbar_init(&acc_empty[s], kOutWarps8);
+      mbar_init(&acc_empty[s], 2 * kOutWarps8);
+      mbar_init(&bias_full[s], 32);
+      mbar_init(&bias_empty[s], kOutWarps8);
+    }
+    for (int s = 0; s < kScaleSlots8; ++s) {
+      mbar_init(&sc_full[s], 32);
+      mbar_init(&sc_empty[s], kOutWarps8);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -179,15 +190,12 @@ __global__ void __launch_bounds__(kThreads8, 1)
     tma_prefetch(&tmA);
     tma_prefetch(&tmW);
   }
-  if (warp == kMmaWarp8) {
-    tmem_alloc(tmem_slot, 512);
-    tmem_relinquish();
-  }
+  if (warp == kMmaWarp8) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
-  __syncthreads();
+  cluster_sync();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  const int n_tiles = p.mt * p.nt;
+  const int n_tiles = p.mt * p.nt, first = blockIdx.x / 2, step = gridDim.x / 2;
   // the launcher checks the compiled register count before the first launch
   if (warp >= kOutWarps8) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther8));
 
@@ -195,34 +203,35 @@ __global__ void __launch_bounds__(kThreads8, 1)
     if (lane == 0) {
       uint32_t c = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
+      for (int tile = first; ok && tile < n_tiles; tile += step) {
         int m0, n0;
         tile8(p, tile, m0, n0);
+        const int a_row = m0 + rank * kM8, w_row = n0 + rank * (tile_cols8(p, n0) / 2);
         for (int kb = 0; kb < p.kb; ++kb, ++c) {
           const int s = c % kStages8;
           if (!(ok = mbar_wait(&empty[s], ((c / kStages8) & 1) ^ 1u, abort_flag, status))) break;
           uint8_t* sa = smem + s * kStage8Bytes;
-          mbar_arrive_expect_tx(&full[s], kStage8Bytes);
-          tma_load_2d(sa, &tmA, &full[s], kb * kK8, m0);
-          tma_load_2d(sa + kA8Bytes, &tmW, &full[s], kb * kK8, n0);
+          const uint32_t bar = map_to_rank(&full[s], 0);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStage8Bytes);
+          tma_load_2d_pair(sa, &tmA, bar, kb * kK8, a_row);
+          tma_load_2d_pair(sa + kA8Bytes, &tmW, bar, kb * kK8, w_row);
         }
       }
-      if (!ok) {  // the copies in flight land before the block's shared memory goes
-        const uint32_t first = c > kStages8 ? c - kStages8 : 0;
-        for (uint32_t i = first; i < c; ++i) {
+      if (!ok && rank == 0) {  // the pair's copies in flight land before its shared memory goes
+        for (uint32_t i = c > kStages8 ? c - kStages8 : 0; i < c; ++i) {
           int none = 0;
           mbar_wait(&full[i % kStages8], (i / kStages8) & 1, &none, nullptr);
         }
       }
     }
   } else if (warp == kMmaWarp8) {
-    if (lane == 0) {
+    if (lane == 0 && rank == 0) {
       uint32_t c = 0;
       bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < n_tiles; tile += gridDim.x) {
+      for (int tile = first; ok && tile < n_tiles; tile += step) {
         int m0, n0;
         tile8(p, tile, m0, n0);
-        const uint32_t idesc = idesc_e4m3_f32(kM8, min(kN8, (p.g.n - n0 + 15) & ~15));
+        const uint32_t idesc = idesc_e4m3_f32(2 * kM8, tile_cols8(p, n0));
         for (int kb = 0; kb < p.kb; ++kb, ++c) {
           const int s = c % kStages8, slot = c & 1;
           if (!(ok = mbar_wait(&acc_empty[slot], ((c >> 1) & 1) ^ 1u, abort_flag, status))) break;
@@ -231,122 +240,211 @@ __global__ void __launch_bounds__(kThreads8, 1)
           const uint32_t sa = smem_u32(smem + s * kStage8Bytes), sb = sa + kA8Bytes;
 #pragma unroll
           for (int k = 0; k < kK8 / 32; ++k)
-            mma_f8_ss(tmem + slot * kN8, sdesc_sw128(sa + k * 32, 1024, 16), sdesc_sw128(sb + k * 32, 1024, 16),
-                      idesc, k != 0 ? 1u : 0u);
-          mma_commit(&empty[s]);
-          mma_commit(&acc_full[slot]);
+            mma_f8_ss_pair(tmem + slot * kN8, sdesc_sw128(sa + k * 32, 1024, 16), sdesc_sw128(sb + k * 32, 1024, 16),
+                           idesc, k != 0 ? 1u : 0u);
+          mma_commit_pair(&empty[s]);
+          mma_commit_pair(&acc_full[slot]);
         }
       }
+    }
+  } else if (warp == kScaleWarp8) {
+    float* ring = reinterpret_cast<float*>(smem + kScale8Off);
+    uint32_t c = 0;
+    bool ok = true;
+    for (int tile = first; ok && tile < n_tiles; tile += step) {
+      int m0, n0;
+      tile8(p, tile, m0, n0);
+      m0 += rank * kM8;
+      const float* a = p.g.a_scales + m0;
+      const float* w = p.g.w_scales + n0 / kBlock8;
+      for (int kb = 0; kb < p.kb; ++kb, ++c, a += p.g.ldas, w += p.g.ldws) {
+        const int s = c % kScaleSlots8;
+        if (!(ok = mbar_wait(&sc_empty[s], ((c / kScaleSlots8) & 1) ^ 1u, abort_flag, status))) break;
+        float* dst = ring + s * kScaleFloats8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = lane + 32 * i;
+          const bool in = m0 + r < p.g.m;
+          cp_async4(dst + r, in ? a + r : p.g.a_scales, in);
+        }
+        if (lane < 2) {
+          const bool in = n0 + lane * kPart8 < p.g.n;
+          cp_async4(dst + kM8 + lane, in ? w + lane : p.g.w_scales, in);
+        }
+        cp_async_arrive(&sc_full[s]);
+      }
+    }
+    cp_async_wait<0>();
+  } else if (warp == kBiasWarp8) {
+    if (p.g.bias) {
+      float* ring = reinterpret_cast<float*>(smem + kBias8Off);
+      uint32_t i = 0;
+      for (int tile = first; tile < n_tiles; tile += step, ++i) {
+        int m0, n0;
+        tile8(p, tile, m0, n0);
+        const int s = i & 1;
+        if (!mbar_wait(&bias_empty[s], ((i >> 1) & 1) ^ 1u, abort_flag, status)) break;
+#pragma unroll
+        for (int j = 0; j < kN8 / 32; ++j) {
+          const int cc = lane + 32 * j;
+          const bool in = n0 + cc < p.g.n;
+          cp_async4(ring + s * kN8 + cc, in ? p.g.bias + n0 + cc : p.g.bias, in);
+        }
+        cp_async_arrive(&bias_full[s]);
+      }
+      cp_async_wait<0>();
     }
   } else if (warp < kOutWarps8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOut8));
     const int quad = warp & 3, part = warp >> 2;
-    const int row = quad * 32 + lane;
+    const uint32_t acc_free = map_to_rank(acc_empty, 0);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16) + part * kPart8;
     uint8_t* bufs = smem + kBuf8Off + warp * 2 * kBuf8Words * 4;
-    float* bias = reinterpret_cast<float*>(smem + kBias8Off) + warp * kPart8;
-    constexpr int E = 128 / sizeof(T);  // output columns per buffer
-    int phase = 0;
-    ScaleStream ss;
-    ss.tile = blockIdx.x;
-    ss.kb = 0;
-    ss.at_tile(p, n_tiles, row, part);
-    float2 s0 = ss.next(p, n_tiles, row, part), s1 = ss.next(p, n_tiles, row, part);
-    uint32_t c = 0;
+    const float* sc = reinterpret_cast<const float*>(smem + kScale8Off);
+    constexpr int E = 128 / sizeof(T);    // output columns per buffer
+    constexpr int kBlocks = kPart8 / E;   // buffers per tile
+    uint32_t c = 0, i_tile = 0;
     bool ok = true;
-    for (int tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+    for (int tile = first; tile < n_tiles; tile += step, ++i_tile) {
       int m0, n0;
       tile8(p, tile, m0, n0);
+      m0 += rank * kM8 + quad * 32;
       n0 += part * kPart8;
-      const int cols = p.g.n - n0;              // columns left from this warp's first
-      const int rows = p.g.m - (m0 + quad * 32);  // rows left from this warp's first
-      const bool live = cols > 0;
+      const int cols = p.g.n - n0;  // columns left from this warp's first
+      const int rows = p.g.m - m0;  // rows left from this warp's first
+      const bool live = cols > 0 && rows > 0;
+      // The residual's first two blocks arrive in the output buffers while the sums form; f32 fetches
+      // the other two once the first two have left.
+      auto fetch_resid = [&](int b) {
+        if (b * E < cols)
+          load_block(bufs + (b & 1) * kBuf8Words * 4,
+                     static_cast<const T*>(p.g.resid) + static_cast<int64_t>(m0) * p.g.ldr + n0 + b * E, p.g.ldr, rows,
+                     cols - b * E, p.resid_vec, lane);
+        cp_async_commit();
+      };
+      if constexpr (O != Out8::Q8) {
+        if (live && p.g.resid) {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+          fetch_resid(0);
+          fetch_resid(1);
+        }
+      }
       float2 acc[kPart8 / 2];
 #pragma unroll
       for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = 0; kb < p.kb; ++kb, ++c) {
-        const int slot = c & 1;
-        const float2 cur = s0;
-        s0 = s1;
-        s1 = ss.next(p, n_tiles, row, part);
+        const int slot = c & 1, ssl = c % kScaleSlots8;
+        if (!(ok = mbar_wait(&sc_full[ssl], (c / kScaleSlots8) & 1, abort_flag, status))) break;
+        const float* sp = sc + ssl * kScaleFloats8;
+        const float fs = sp[quad * 32 + lane] * sp[kM8 + part];
+        const float2 f = make_float2(fs, fs);
         if (!(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status))) break;
         tc_fence_after();
         if (live) {
           const uint32_t t = tm + slot * kN8;
-          const float2 f = make_float2(cur.x * cur.y, cur.x * cur.y);
-          uint32_t va[32], vb[32];
-          tmem_ld32(t, va);
-          tmem_ld_wait(va);
+          uint32_t v[2][32];
+          tmem_ld32(t, v[0]);
+          tmem_ld_wait(v[0]);
 #pragma unroll
-          for (int b = 0; b < kPart8 / 32; b += 2) {
-            tmem_ld32(t + 32 * (b + 1), vb);
+          for (int b = 0; b < kPart8 / 32; ++b) {
+            if (b + 1 < kPart8 / 32) tmem_ld32(t + 32 * (b + 1), v[(b + 1) & 1]);
+            if (b + 1 == kPart8 / 32) {  // all read: the accumulator is free before the last multiplications
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive_cluster(acc_free + slot * 8);
+                mbar_arrive(&sc_empty[ssl]);
+              }
+            }
 #pragma unroll
             for (int i = 0; i < 16; ++i)
-              acc[16 * b + i] = __ffma2_rn(make_float2(__uint_as_float(va[2 * i]), __uint_as_float(va[2 * i + 1])), f,
-                                           acc[16 * b + i]);
-            tmem_ld_wait(vb);
-            if (b + 2 < kPart8 / 32) tmem_ld32(t + 32 * (b + 2), va);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              acc[16 * (b + 1) + i] = __ffma2_rn(
-                  make_float2(__uint_as_float(vb[2 * i]), __uint_as_float(vb[2 * i + 1])), f, acc[16 * (b + 1) + i]);
-            if (b + 2 < kPart8 / 32) tmem_ld_wait(va);
+              acc[16 * b + i] =
+                  __ffma2_rn(make_float2(__uint_as_float(v[b & 1][2 * i]), __uint_as_float(v[b & 1][2 * i + 1])), f,
+                             acc[16 * b + i]);
+            if (b + 1 < kPart8 / 32) tmem_ld_wait(v[(b + 1) & 1]);
+          }
+        } else {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_cluster(acc_free + slot * 8);
+            mbar_arrive(&sc_empty[ssl]);
           }
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&acc_empty[slot]);
       }
       if (!ok) break;
-      if (!live || rows <= 0) continue;
       // ---------------- output ----------------
       if (p.g.bias) {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int cc = lane + 32 * i;
-          bias[cc] = cc < cols ? __ldg(p.g.bias + n0 + cc) : 0.0f;
-        }
-        __syncwarp();
+        const int bs = i_tile & 1;
+        if (!(ok = mbar_wait(&bias_full[bs], (i_tile >> 1) & 1, abort_flag, status))) break;
+        const float* bias = reinterpret_cast<const float*>(smem + kBias8Off) + bs * kN8 + part * kPart8;
 #pragma unroll
         for (int i = 0; i < kPart8 / 4; ++i) {
-          const float4 v = lds4f(bias + 4 * i);
+          const float4 v = *reinterpret_cast<const float4*>(bias + 4 * i);
           acc[2 * i] = __fadd2_rn(acc[2 * i], make_float2(v.x, v.y));
           acc[2 * i + 1] = __fadd2_rn(acc[2 * i + 1], make_float2(v.z, v.w));
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bias_empty[bs]);
       }
+      if (!live) continue;
       float inv = 0.0f;
       if constexpr (O == Out8::Q8) {
         uint32_t top = 0;
+        if (cols >= kPart8) {
 #pragma unroll
-        for (int i = 0; i < kPart8 / 2; ++i) {
-          acc[i] = gelu_as2(acc[i]);
-          if (2 * i < cols) top = max(top, mag_bits(acc[i].x));
-          if (2 * i + 1 < cols) top = max(top, mag_bits(acc[i].y));
+          for (int i = 0; i < kPart8 / 2; ++i) {
+            acc[i] = gelu8(acc[i]);
+            top = max(top, max(mag_bits(acc[i].x), mag_bits(acc[i].y)));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPart8 / 2; ++i) {
+            acc[i] = gelu8(acc[i]);
+            if (2 * i < cols) top = max(top, mag_bits(acc[i].x));
+            if (2 * i + 1 < cols) top = max(top, mag_bits(acc[i].y));
+          }
         }
         const Scale8 s = scale8(top);
         inv = s.inv;
-        if (lane < rows) p.g.scales[static_cast<int64_t>(n0 / kBlock8) * p.g.lds + m0 + row] = s.s;
+        if (lane < rows) p.g.scales[static_cast<int64_t>(n0 / kBlock8) * p.g.lds + m0 + lane] = s.s;
       }
 #pragma unroll
-      for (int b = 0; b < kPart8 / E; ++b) {
+      for (int b = 0; b < kBlocks; ++b) {
         const int cb = b * E;
         if (cb >= cols) break;
-        uint8_t* buf = bufs + (phase++ & 1) * kBuf8Words * 4;
-        if (lane == 0) tma_store_wait_read<1>();
-        __syncwarp();
+        uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
         uint32_t w[32];
         if constexpr (O == Out8::Q8) {
+          if (lane == 0) tma_store_wait_read<0>();
+          __syncwarp();
+          const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-          for (int i = 0; i < 32; ++i)
-            w[i] = e4m3x4(acc[2 * i].x * inv, acc[2 * i].y * inv, acc[2 * i + 1].x * inv, acc[2 * i + 1].y * inv);
+          for (int i = 0; i < 32; ++i) {
+            const float2 x = __fmul2_rn(acc[2 * i], inv2), y = __fmul2_rn(acc[2 * i + 1], inv2);
+            w[i] = e4m3x4(x.x, x.y, y.x, y.y);
+          }
         } else {
           if (p.g.resid) {
-            load_block(buf, static_cast<const T*>(p.g.resid) + static_cast<int64_t>(m0 + quad * 32) * p.g.ldr + n0 + cb,
-                       p.g.ldr, rows, cols - cb, p.resid_vec, lane);
-            cp_async_wait_all();
-            __syncwarp();
+            if (b == 2) {
+              if (lane == 0) tma_store_wait_read<0>();
+              __syncwarp();
+              fetch_resid(2);
+              fetch_resid(3);
+            }
+            if (b & 1)
+              cp_async_wait<0>();
+            else
+              cp_async_wait<1>();
+          } else if (lane == 0) {
+            // the last tile may have stopped at either buffer
+            if (b == 0)
+              tma_store_wait_read<0>();
+            else
+              tma_store_wait_read<1>();
           }
+          __syncwarp();
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
             uint4 r = make_uint4(0u, 0u, 0u, 0u);
@@ -365,7 +463,6 @@ __global__ void __launch_bounds__(kThreads8, 1)
               }
             }
           }
-          __syncwarp();
         }
 #pragma unroll
         for (int v = 0; v < 8; ++v)
@@ -375,32 +472,54 @@ __global__ void __launch_bounds__(kThreads8, 1)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            tma_store_2d(&tmOut, buf, n0 + cb, m0 + quad * 32);
+            tma_store_2d(&tmOut, buf, n0 + cb, m0);
             tma_store_commit();
           }
         } else {
           __syncwarp();
           T* dst = O == Out8::Q8 ? reinterpret_cast<T*>(p.g.q) : static_cast<T*>(p.g.out);
           const int64_t ld = O == Out8::Q8 ? p.g.ldq : p.g.ldo;
-          store_block(buf, dst + static_cast<int64_t>(m0 + quad * 32) * ld + n0 + cb, ld, rows, cols - cb, lane);
+          store_block(buf, dst + static_cast<int64_t>(m0) * ld + n0 + cb, ld, rows, cols - cb, lane);
+          __syncwarp();
         }
       }
     }
+    cp_async_wait<0>();
     if (lane == 0) tma_store_wait_all();
     __syncwarp();
   }
   tc_fence_before();
-  __syncthreads();
+  __syncwarp();
+  cluster_sync();  // neither CTA goes while the other may still reach its shared memory
   if (warp == kMmaWarp8) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
-static int sm_count() {
+// Pairs that run at one time on the current device.
+static int resident_pairs(const void* kernel) {
+  static std::atomic<int> known[64];
   int dev = 0, n = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return 148;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+  if ((n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
+  int sms = 0;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sms / 2 * 2);
+  cfg.blockDim = dim3(kThreads8);
+  cfg.dynamicSmemBytes = kSmem8;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 2;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+    cudaGetLastError();
+    n = sms / 2 > 0 ? sms / 2 : 1;
+  }
+  known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 
@@ -418,9 +537,9 @@ static cudaError_t launch8(const CUtensorMap& ta, const CUtensorMap& tw, const C
     return fa.numRegs >= kLaunchRegs8 ? cudaSuccess : cudaErrorInvalidConfiguration;
   });
   if (e != cudaSuccess) return e;
-  const int tiles = p.mt * p.nt, sms = sm_count();
+  const int tiles = p.mt * p.nt, pairs = resident_pairs(reinterpret_cast<const void*>(gemm8_kernel<O>));
   count_launch();
-  gemm8_kernel<O><<<tiles < sms ? tiles : sms, kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
+  gemm8_kernel<O><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
   return cudaGetLastError();
 }
 
@@ -428,12 +547,12 @@ cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
   CUtensorMap ta, tw, to;
   Params8 p;
   p.g = g;
-  p.mt = (g.m + kM8 - 1) / kM8;
+  p.mt = (g.m + 2 * kM8 - 1) / (2 * kM8);
   p.nt = (g.n + kN8 - 1) / kN8;
-  p.group = 8;
+  p.per = make_fastdiv(static_cast<uint32_t>(kGroup8 * p.nt), static_cast<uint64_t>(p.mt) * p.nt);
   p.kb = (g.k + kK8 - 1) / kK8;
   cudaError_t e = make_map_2d(&ta, g.a, g.k, g.m, g.lda, kK8, kM8, MapElem::U8);
-  if (e == cudaSuccess) e = make_map_2d(&tw, g.w, g.k, g.n, g.ldw, kK8, kN8, MapElem::U8);
+  if (e == cudaSuccess) e = make_map_2d(&tw, g.w, g.k, g.n, g.ldw, kK8, kN8 / 2, MapElem::U8);
   if (e != cudaSuccess) return e;
   const int size = !g.out ? 1 : g.out_type == Elem::F32 ? 4 : 2;
   const void* dst = g.out ? g.out : g.q;
