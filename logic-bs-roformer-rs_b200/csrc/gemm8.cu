@@ -39,7 +39,7 @@ constexpr int kOutWarps8 = 8;
 constexpr int kPart8 = kN8 / 2;                             // columns per output warp
 constexpr int kBuf8Words = 1024;                            // 32 rows x 128 bytes; two per output warp
 constexpr int kBuf8Off = kStages8 * kStage8Bytes;
-constexpr int kScaleSlots8 = 8;                             // K-blocks
+constexpr int kScaleSlots8 = 8, kScaleAhead8 = 4;           // K-blocks in the ring, and loaded ahead
 constexpr int kScaleFloats8 = kM8 + 4;                      // a slot: 128 rows' scales, then W's of the two parts
 constexpr int kScale8Off = kBuf8Off + kOutWarps8 * 2 * kBuf8Words * 4;
 constexpr int kBias8Off = kScale8Off + kScaleSlots8 * kScaleFloats8 * 4;  // two tiles' bias
@@ -145,6 +145,15 @@ __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t 
 // Columns of the pair's tile that the MMA computes: whole 32s, 16 per CTA's half of W.
 __device__ __forceinline__ int tile_cols8(const Params8& p, int n0) { return min(kN8, (p.g.n - n0 + 31) & ~31); }
 
+// 32 columns of a block's sums, times the block's factor, added to the totals.
+template <int B>
+__device__ __forceinline__ void add_scaled(float2 (&acc)[kPart8 / 2], const uint32_t (&v)[32], float2 f) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i)
+    acc[16 * B + i] =
+        __ffma2_rn(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f, acc[16 * B + i]);
+}
+
 template <Out8 O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
@@ -155,11 +164,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
   const uint32_t rank = cluster_rank();
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBar8Off);  // CTA 0's: both CTAs' loads
   uint64_t* empty = full + kStages8;
-  uint64_t* acc_full = empty + kStages8;  // [2]
+  uint64_t* acc_full = empty + kStages8;  // [2], the block's sums and its scales
   uint64_t* acc_empty = acc_full + 2;     // [2], CTA 0's: both CTAs' output warps
-  uint64_t* sc_full = acc_empty + 2;                // [kScaleSlots8], 32 lanes' copies
-  uint64_t* sc_empty = sc_full + kScaleSlots8;      // [kScaleSlots8]
-  uint64_t* bias_full = sc_empty + kScaleSlots8;    // [2], 32 lanes' copies
+  uint64_t* bias_full = acc_empty + 2;    // [2], 32 lanes' copies
   uint64_t* bias_empty = bias_full + 2;             // [2]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bias_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -174,14 +181,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       mbar_init(&empty[s], 1);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&acc_full[s], 1);
+      mbar_init(&acc_full[s], 2);
       mbar_init(&acc_empty[s], 2 * kOutWarps8);
       mbar_init(&bias_full[s], 32);
       mbar_init(&bias_empty[s], kOutWarps8);
-    }
-    for (int s = 0; s < kScaleSlots8; ++s) {
-      mbar_init(&sc_full[s], 32);
-      mbar_init(&sc_empty[s], kOutWarps8);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -234,36 +237,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         const uint32_t idesc = idesc_e4m3_f32(2 * kM8, tile_cols8(p, n0));
         for (int kb = 0; kb < p.kb; ++kb, ++c) {
           const int s = c % kStages8, slot = c & 1;
-          if (!(ok = mbar_wait(&acc_empty[slot], ((c >> 1) & 1) ^ 1u, abort_flag, status))) break;
+          // the accumulator, waited for last, is what the MMAs usually wait for
           if (!(ok = mbar_wait(&full[s], (c / kStages8) & 1, abort_flag, status))) break;
+          if (!(ok = mbar_wait(&acc_empty[slot], ((c >> 1) & 1) ^ 1u, abort_flag, status))) break;
           tc_fence_after();
           const uint32_t sa = smem_u32(smem + s * kStage8Bytes), sb = sa + kA8Bytes;
 #pragma unroll
           for (int k = 0; k < kK8 / 32; ++k)
             mma_f8_ss_pair(tmem + slot * kN8, sdesc_sw128(sa + k * 32, 1024, 16), sdesc_sw128(sb + k * 32, 1024, 16),
                            idesc, k != 0 ? 1u : 0u);
-          mma_commit_pair(&empty[s]);
           mma_commit_pair(&acc_full[slot]);
+          mma_commit_pair(&empty[s]);
         }
       }
     }
   } else if (warp == kScaleWarp8) {
+    // The copies for block c + kScaleAhead8 are issued once block c - 2's sums are complete: the accumulator
+    // of block c - 2 was then free, so every output warp is done with block c - 4, whose place they take.
     float* ring = reinterpret_cast<float*>(smem + kScale8Off);
-    uint32_t c = 0;
-    bool ok = true;
-    for (int tile = first; ok && tile < n_tiles; tile += step) {
-      int m0, n0;
-      tile8(p, tile, m0, n0);
-      m0 += rank * kM8;
-      const float* a = p.g.a_scales + m0;
-      const float* w = p.g.w_scales + n0 / kBlock8;
-      for (int kb = 0; kb < p.kb; ++kb, ++c, a += p.g.ldas, w += p.g.ldws) {
-        const int s = c % kScaleSlots8;
-        if (!(ok = mbar_wait(&sc_empty[s], ((c / kScaleSlots8) & 1) ^ 1u, abort_flag, status))) break;
-        float* dst = ring + s * kScaleFloats8;
+    uint32_t issued = 0;
+    int i_tile = first, i_kb = 0, m0 = 0, n0 = 0;
+    const float *a = nullptr, *w = nullptr;
+    auto issue = [&]() {
+      if (i_tile < n_tiles) {
+        if (i_kb == 0) {
+          tile8(p, i_tile, m0, n0);
+          m0 += rank * kM8;
+          a = p.g.a_scales + m0;
+          w = p.g.w_scales + n0 / kBlock8;
+        }
+        float* dst = ring + issued % kScaleSlots8 * kScaleFloats8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = lane + 32 * i;
+        for (int j = 0; j < 4; ++j) {
+          const int r = lane + 32 * j;
           const bool in = m0 + r < p.g.m;
           cp_async4(dst + r, in ? a + r : p.g.a_scales, in);
         }
@@ -271,8 +277,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
           const bool in = n0 + lane * kPart8 < p.g.n;
           cp_async4(dst + kM8 + lane, in ? w + lane : p.g.w_scales, in);
         }
-        cp_async_arrive(&sc_full[s]);
+        a += p.g.ldas;
+        w += p.g.ldws;
+        if (++i_kb == p.kb) {
+          i_kb = 0;
+          i_tile += step;
+        }
+        ++issued;
       }
+      cp_async_commit();
+    };
+    for (int i = 0; i < kScaleAhead8; ++i) issue();
+    for (uint32_t c = 0; c < issued; ++c) {
+      cp_async_wait<kScaleAhead8 - 1>();
+      __syncwarp();
+      const int slot = c & 1;
+      if (c >= 2 && !mbar_wait(&acc_full[slot], ((c - 2) >> 1) & 1, abort_flag, status)) break;
+      if (lane == 0) mbar_arrive(&acc_full[slot]);
+      issue();
     }
     cp_async_wait<0>();
   } else if (warp == kBiasWarp8) {
@@ -334,43 +356,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
 #pragma unroll
       for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = 0; kb < p.kb; ++kb, ++c) {
-        const int slot = c & 1, ssl = c % kScaleSlots8;
-        if (!(ok = mbar_wait(&sc_full[ssl], (c / kScaleSlots8) & 1, abort_flag, status))) break;
-        const float* sp = sc + ssl * kScaleFloats8;
-        const float fs = sp[quad * 32 + lane] * sp[kM8 + part];
-        const float2 f = make_float2(fs, fs);
+        const int slot = c & 1;
         if (!(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status))) break;
         tc_fence_after();
+        const float* sp = sc + c % kScaleSlots8 * kScaleFloats8;
         if (live) {
+          // two 32-column loads in flight, two waits a block: the block's latency, not its arithmetic, sets the pace
           const uint32_t t = tm + slot * kN8;
-          uint32_t v[2][32];
-          tmem_ld32(t, v[0]);
-          tmem_ld_wait(v[0]);
-#pragma unroll
-          for (int b = 0; b < kPart8 / 32; ++b) {
-            if (b + 1 < kPart8 / 32) tmem_ld32(t + 32 * (b + 1), v[(b + 1) & 1]);
-            if (b + 1 == kPart8 / 32) {  // all read: the accumulator is free before the last multiplications
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) {
-                mbar_arrive_cluster(acc_free + slot * 8);
-                mbar_arrive(&sc_empty[ssl]);
-              }
-            }
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              acc[16 * b + i] =
-                  __ffma2_rn(make_float2(__uint_as_float(v[b & 1][2 * i]), __uint_as_float(v[b & 1][2 * i + 1])), f,
-                             acc[16 * b + i]);
-            if (b + 1 < kPart8 / 32) tmem_ld_wait(v[(b + 1) & 1]);
-          }
+          uint32_t va[32], vb[32];
+          tmem_ld32(t, va);
+          tmem_ld32(t + 32, vb);
+          const float fs = sp[quad * 32 + lane] * sp[kM8 + part];
+          const float2 f = make_float2(fs, fs);
+          tmem_ld_wait(va);
+          tmem_ld_wait(vb);
+          add_scaled<0>(acc, va, f);
+          tmem_ld32(t + 64, va);
+          add_scaled<1>(acc, vb, f);
+          tmem_ld32(t + 96, vb);
+          tmem_ld_wait(va);
+          tmem_ld_wait(vb);
+          tc_fence_before();  // all read: the accumulator is free before the last multiplications
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cluster(acc_free + slot * 8);
+          add_scaled<2>(acc, va, f);
+          add_scaled<3>(acc, vb, f);
         } else {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) {
-            mbar_arrive_cluster(acc_free + slot * 8);
-            mbar_arrive(&sc_empty[ssl]);
-          }
+          if (lane == 0) mbar_arrive_cluster(acc_free + slot * 8);
         }
       }
       if (!ok) break;
