@@ -228,9 +228,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       }
     }
   } else if (warp == kMmaWarp8) {
-    if (lane == 0 && rank == 0) {
+    if (rank == 0) {  // the whole warp, so that descriptors and addresses stay uniform; one lane issues
+      const uint32_t leader = elect_one();
       uint32_t c = 0;
-      bool ok = true;
+      bool ok = true, loaded = false;  // loaded: block c's operands were seen to have landed
       for (int tile = first; ok && tile < n_tiles; tile += step) {
         int m0, n0;
         tile8(p, tile, m0, n0);
@@ -238,16 +239,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         for (int kb = 0; kb < p.kb; ++kb, ++c) {
           const int s = c % kStages8, slot = c & 1;
           // the accumulator, waited for last, is what the MMAs usually wait for
-          if (!(ok = mbar_wait(&full[s], (c / kStages8) & 1, abort_flag, status))) break;
+          if (!__all_sync(0xffffffffu, loaded) &&
+              !(ok = mbar_wait(&full[s], (c / kStages8) & 1, abort_flag, status)))
+            break;
           if (!(ok = mbar_wait(&acc_empty[slot], ((c >> 1) & 1) ^ 1u, abort_flag, status))) break;
+          __syncwarp();
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kStage8Bytes), sb = sa + kA8Bytes;
+          const uint64_t da = sdesc_sw128(smem_u32(smem) + s * kStage8Bytes, 1024, 16);
 #pragma unroll
-          for (int k = 0; k < kK8 / 32; ++k)
-            mma_f8_ss_pair(tmem + slot * kN8, sdesc_sw128(sa + k * 32, 1024, 16), sdesc_sw128(sb + k * 32, 1024, 16),
-                           idesc, k != 0 ? 1u : 0u);
-          mma_commit_pair(&acc_full[slot]);
-          mma_commit_pair(&empty[s]);
+          for (int k = 0; k < kK8 / 32; ++k)  // 32 bytes along a row, in the descriptors' units of 16
+            mma_f8_ss_pair(leader, tmem + slot * kN8, da + k * 2, da + kA8Bytes / 16 + k * 2, idesc, k != 0 ? 1u : 0u);
+          mma_commit_pair(leader, &acc_full[slot]);
+          mma_commit_pair(leader, &empty[s]);
+          loaded = mbar_test(&full[(c + 1) % kStages8], ((c + 1) / kStages8) & 1);
         }
       }
     }
@@ -326,7 +330,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     constexpr int E = 128 / sizeof(T);    // output columns per buffer
     constexpr int kBlocks = kPart8 / E;   // buffers per tile
     uint32_t c = 0, i_tile = 0;
-    bool ok = true;
+    const uint32_t leader = elect_one();
+    bool ok = true, summed = false;  // summed: block c's sums were seen to be complete
     for (int tile = first; tile < n_tiles; tile += step, ++i_tile) {
       int m0, n0;
       tile8(p, tile, m0, n0);
@@ -357,34 +362,37 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       for (int kb = 0; kb < p.kb; ++kb, ++c) {
         const int slot = c & 1;
-        if (!(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status))) break;
+        if (!__all_sync(0xffffffffu, summed) &&
+            !(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status)))
+          break;
+        __syncwarp();
         tc_fence_after();
         const float* sp = sc + c % kScaleSlots8 * kScaleFloats8;
         if (live) {
           // two 32-column loads in flight, two waits a block: the block's latency, not its arithmetic, sets the pace
           const uint32_t t = tm + slot * kN8;
           uint32_t va[32], vb[32];
-          tmem_ld32(t, va);
-          tmem_ld32(t + 32, vb);
+          tmem_ld32_converged(t, va);
+          tmem_ld32_converged(t + 32, vb);
           const float fs = sp[quad * 32 + lane] * sp[kM8 + part];
           const float2 f = make_float2(fs, fs);
           tmem_ld_wait(va);
           tmem_ld_wait(vb);
           add_scaled<0>(acc, va, f);
-          tmem_ld32(t + 64, va);
+          tmem_ld32_converged(t + 64, va);
           add_scaled<1>(acc, vb, f);
-          tmem_ld32(t + 96, vb);
+          tmem_ld32_converged(t + 96, vb);
           tmem_ld_wait(va);
           tmem_ld_wait(vb);
           tc_fence_before();  // all read: the accumulator is free before the last multiplications
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_free + slot * 8);
+          mbar_arrive_cluster(leader, acc_free + slot * 8);
+          summed = mbar_test(&acc_full[slot ^ 1], ((c + 1) >> 1) & 1);
           add_scaled<2>(acc, va, f);
           add_scaled<3>(acc, vb, f);
         } else {
           tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(acc_free + slot * 8);
+          mbar_arrive_cluster(leader, acc_free + slot * 8);
+          summed = false;
         }
       }
       if (!ok) break;
