@@ -12,15 +12,17 @@
 
 namespace lbrr {
 
+__device__ __forceinline__ float neg_abs(float x) { return __uint_as_float(__float_as_uint(x) | 0x80000000u); }
+
 __device__ __forceinline__ float2 gelu8(float2 x) {
-  const float2 a = f2(fabsf(x.x), fabsf(x.y));
-  float2 p = __ffma2_rn(a, f2(-5.188582732e-04f, -5.188582732e-04f), f2(7.387199601e-03f, 7.387199601e-03f));
-  p = __ffma2_rn(p, a, f2(-5.253801530e-02f, -5.253801530e-02f));
-  p = __ffma2_rn(p, a, f2(-4.592766851e-01f, -4.592766851e-01f));
-  p = __ffma2_rn(p, a, f2(-1.151083144e+00f, -1.151083144e+00f));
-  p = __ffma2_rn(p, a, f2(-1.000000836e+00f, -1.000000836e+00f));
+  const float2 n = f2(neg_abs(x.x), neg_abs(x.y));  // -a; the odd coefficients change sign
+  float2 p = __ffma2_rn(n, f2(5.188582732e-04f, 5.188582732e-04f), f2(7.387199601e-03f, 7.387199601e-03f));
+  p = __ffma2_rn(p, n, f2(5.253801530e-02f, 5.253801530e-02f));
+  p = __ffma2_rn(p, n, f2(-4.592766851e-01f, -4.592766851e-01f));
+  p = __ffma2_rn(p, n, f2(1.151083144e+00f, 1.151083144e+00f));
+  p = __ffma2_rn(p, n, f2(-1.000000836e+00f, -1.000000836e+00f));
   const float2 t = f2(ex2_approx(p.x), ex2_approx(p.y));
-  return __ffma2_rn(f2(-a.x, -a.y), t, f2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+  return __ffma2_rn(n, t, f2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
 }
 
 }  // namespace lbrr

@@ -147,7 +147,8 @@ __device__ __forceinline__ int tile_cols8(const Params8& p, int n0) { return min
 
 // 32 columns of a block's sums, times the block's factor, added to the totals.
 template <int B>
-__device__ __forceinline__ void add_scaled(float2 (&acc)[kPart8 / 2], const uint32_t (&v)[32], float2 f) {
+__device__ __forceinline__ void add_scaled(float2 (&acc)[kPart8 / 2], const uint32_t (&v)[32], float s) {
+  const float2 f = make_float2(s, s);
 #pragma unroll
   for (int i = 0; i < 16; ++i)
     acc[16 * B + i] =
@@ -331,7 +332,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     constexpr int kBlocks = kPart8 / E;   // buffers per tile
     uint32_t c = 0, i_tile = 0;
     const uint32_t leader = elect_one();
-    bool ok = true, summed = false;  // summed: block c's sums were seen to be complete
+    bool ok = true;
     for (int tile = first; tile < n_tiles; tile += step, ++i_tile) {
       int m0, n0;
       tile8(p, tile, m0, n0);
@@ -358,152 +359,172 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         }
       }
       float2 acc[kPart8 / 2];
-#pragma unroll
-      for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
-      for (int kb = 0; kb < p.kb; ++kb, ++c) {
-        const int slot = c & 1;
-        if (!__all_sync(0xffffffffu, summed) &&
-            !(ok = mbar_wait(&acc_full[slot], (c >> 1) & 1, abort_flag, status)))
-          break;
-        __syncwarp();
-        tc_fence_after();
-        const float* sp = sc + c % kScaleSlots8 * kScaleFloats8;
-        if (live) {
-          // two 32-column loads in flight, two waits a block: the block's latency, not its arithmetic, sets the pace
-          const uint32_t t = tm + slot * kN8;
-          uint32_t va[32], vb[32];
-          tmem_ld32_converged(t, va);
-          tmem_ld32_converged(t + 32, vb);
-          const float fs = sp[quad * 32 + lane] * sp[kM8 + part];
-          const float2 f = make_float2(fs, fs);
-          tmem_ld_wait(va);
-          tmem_ld_wait(vb);
-          add_scaled<0>(acc, va, f);
-          tmem_ld32_converged(t + 64, va);
-          add_scaled<1>(acc, vb, f);
-          tmem_ld32_converged(t + 96, vb);
-          tmem_ld_wait(va);
-          tmem_ld_wait(vb);
-          tc_fence_before();  // all read: the accumulator is free before the last multiplications
-          mbar_arrive_cluster(leader, acc_free + slot * 8);
-          summed = mbar_test(&acc_full[slot ^ 1], ((c + 1) >> 1) & 1);
-          add_scaled<2>(acc, va, f);
-          add_scaled<3>(acc, vb, f);
-        } else {
-          tc_fence_before();
-          mbar_arrive_cluster(leader, acc_free + slot * 8);
-          summed = false;
-        }
-      }
-      if (!ok) break;
-      // ---------------- output ----------------
-      if (p.g.bias) {
+      if (p.g.bias) {  // the totals start from the bias
         const int bs = i_tile & 1;
         if (!(ok = mbar_wait(&bias_full[bs], (i_tile >> 1) & 1, abort_flag, status))) break;
         const float* bias = reinterpret_cast<const float*>(smem + kBias8Off) + bs * kN8 + part * kPart8;
 #pragma unroll
         for (int i = 0; i < kPart8 / 4; ++i) {
           const float4 v = *reinterpret_cast<const float4*>(bias + 4 * i);
-          acc[2 * i] = __fadd2_rn(acc[2 * i], make_float2(v.x, v.y));
-          acc[2 * i + 1] = __fadd2_rn(acc[2 * i + 1], make_float2(v.z, v.w));
+          acc[2 * i] = make_float2(v.x, v.y);
+          acc[2 * i + 1] = make_float2(v.z, v.w);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&bias_empty[bs]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kPart8 / 2; ++i) acc[i] = make_float2(0.0f, 0.0f);
       }
+      // The block's latency, not its arithmetic, sets the pace: two 32-column loads are in flight, two waits a
+      // block, and the next block's first loads start before this block's last multiplications when its sums
+      // are already there.
+      uint32_t va[32], vb[32];
+      float f = 0.0f;
+      auto begin = [&](bool a, bool b) {  // first loads of block c, whose barrier has completed
+        if (a) {
+          tc_fence_after();
+          const float* sp = sc + c % kScaleSlots8 * kScaleFloats8;
+          f = sp[quad * 32 + lane] * sp[kM8 + part];
+          tmem_ld32_converged(tm + (c & 1) * kN8, va);
+        }
+        if (b) tmem_ld32_converged(tm + (c & 1) * kN8 + 32, vb);
+      };
+      auto wait_sums = [&]() {
+        ok = mbar_wait(&acc_full[c & 1], (c >> 1) & 1, abort_flag, status);
+        __syncwarp();
+        return ok;
+      };
+      if (!wait_sums()) break;
+      if (live) {
+        begin(true, true);
+        for (int kb = 0;;) {
+          const uint32_t t = tm + (c & 1) * kN8, freed = acc_free + (c & 1) * 8;
+          const float f0 = f;
+          tmem_ld_wait(va);
+          tmem_ld_wait(vb);
+          add_scaled<0>(acc, va, f0);
+          tmem_ld32_converged(t + 64, va);
+          add_scaled<1>(acc, vb, f0);
+          tmem_ld32_converged(t + 96, vb);
+          ++c;
+          const bool more = ++kb < p.kb;
+          const bool ready = more && mbar_test(&acc_full[c & 1], (c >> 1) & 1);
+          tmem_ld_wait(va);
+          tmem_ld_wait(vb);
+          tc_fence_before();  // all read: the accumulator is free before the last multiplications
+          mbar_arrive_cluster(leader, freed);
+          if (__all_sync(0xffffffffu, ready)) {
+            add_scaled<2>(acc, va, f0);
+            begin(true, false);
+            add_scaled<3>(acc, vb, f0);
+            begin(false, true);
+          } else {
+            add_scaled<2>(acc, va, f0);
+            add_scaled<3>(acc, vb, f0);
+            if (!more || !wait_sums()) break;
+            begin(true, true);
+          }
+        }
+      } else {
+        for (int kb = 0;;) {
+          tc_fence_before();
+          mbar_arrive_cluster(leader, acc_free + (c & 1) * 8);
+          ++c;
+          if (++kb == p.kb || !wait_sums()) break;
+        }
+      }
+      if (!ok) break;
+      // ---------------- output ----------------
       if (!live) continue;
       float inv = 0.0f;
       if constexpr (O == Out8::Q8) {
-        uint32_t top = 0;
+        float top = 0.0f;
         if (cols >= kPart8) {
 #pragma unroll
           for (int i = 0; i < kPart8 / 2; ++i) {
             acc[i] = gelu8(acc[i]);
-            top = max(top, max(mag_bits(acc[i].x), mag_bits(acc[i].y)));
+            top = max_mag3(top, acc[i].x, acc[i].y);
           }
         } else {
 #pragma unroll
           for (int i = 0; i < kPart8 / 2; ++i) {
             acc[i] = gelu8(acc[i]);
-            if (2 * i < cols) top = max(top, mag_bits(acc[i].x));
-            if (2 * i + 1 < cols) top = max(top, mag_bits(acc[i].y));
+            top = max_mag3(top, 2 * i < cols ? acc[i].x : 0.0f, 2 * i + 1 < cols ? acc[i].y : 0.0f);
           }
         }
-        const Scale8 s = scale8(top);
+        const Scale8 s = scale8(__float_as_uint(top));
         inv = s.inv;
         if (lane < rows) p.g.scales[static_cast<int64_t>(n0 / kBlock8) * p.g.lds + m0 + lane] = s.s;
       }
+      // two buffers at a time: written, published to the TMA stores with one fence, stored
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b) {
-        const int cb = b * E;
-        if (cb >= cols) break;
-        uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
-        uint32_t w[32];
-        if constexpr (O == Out8::Q8) {
+      for (int b0 = 0; b0 < kBlocks; b0 += 2) {
+        if (b0 * E >= cols) break;
+        if (O == Out8::Q8 || !p.g.resid || b0 > 0) {  // the buffers' last stores have read them
           if (lane == 0) tma_store_wait_read<0>();
           __syncwarp();
-          const float2 inv2 = make_float2(inv, inv);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            const float2 x = __fmul2_rn(acc[2 * i], inv2), y = __fmul2_rn(acc[2 * i + 1], inv2);
-            w[i] = e4m3x4(x.x, x.y, y.x, y.y);
-          }
-        } else {
+        }
+        if constexpr (O != Out8::Q8) {
           if (p.g.resid) {
-            if (b == 2) {
-              if (lane == 0) tma_store_wait_read<0>();
-              __syncwarp();
-              fetch_resid(2);
-              fetch_resid(3);
+            if (b0 > 0) {
+              fetch_resid(b0);
+              fetch_resid(b0 + 1);
             }
-            if (b & 1)
-              cp_async_wait<0>();
-            else
-              cp_async_wait<1>();
-          } else if (lane == 0) {
-            // the last tile may have stopped at either buffer
-            if (b == 0)
-              tma_store_wait_read<0>();
-            else
-              tma_store_wait_read<1>();
+            cp_async_wait<0>();
+            __syncwarp();
           }
-          __syncwarp();
+        }
+#pragma unroll
+        for (int b = b0; b < (b0 + 2 < kBlocks ? b0 + 2 : kBlocks); ++b) {
+          uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
-            uint4 r = make_uint4(0u, 0u, 0u, 0u);
-            if (p.g.resid) r = *reinterpret_cast<const uint4*>(buf + swz(lane, v * 16));
-            const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+            uint4* at = reinterpret_cast<uint4*>(buf + swz(lane, v * 16));
+            uint32_t w[4];
+            if constexpr (O == Out8::Q8) {
+              const float2 inv2 = make_float2(inv, inv);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              if constexpr (O == Out8::F32) {
-                const float2 a = acc[(cb + v * 4 + i) / 2];
-                const float h = (i & 1) ? a.y : a.x;
-                w[v * 4 + i] = __float_as_uint(p.g.resid ? h + __uint_as_float(rw[i]) : h);
-              } else {
-                float2 a = acc[cb / 2 + v * 4 + i];
-                if (p.g.resid) a = __fadd2_rn(a, unpack2(rw[i], T()));
-                w[v * 4 + i] = pack2(a.x, a.y, T());
+              for (int i = 0; i < 4; ++i) {
+                const float2 x = __fmul2_rn(acc[8 * v + 2 * i], inv2), y = __fmul2_rn(acc[8 * v + 2 * i + 1], inv2);
+                w[i] = e4m3x4(x.x, x.y, y.x, y.y);
+              }
+            } else {
+              uint4 r = make_uint4(0u, 0u, 0u, 0u);
+              if (p.g.resid) r = *at;
+              const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if constexpr (O == Out8::F32) {
+                  const float2 a = acc[(b * E + v * 4 + i) / 2];
+                  const float h = (i & 1) ? a.y : a.x;
+                  w[i] = __float_as_uint(p.g.resid ? h + __uint_as_float(rw[i]) : h);
+                } else {
+                  float2 a = acc[b * E / 2 + v * 4 + i];
+                  if (p.g.resid) a = __fadd2_rn(a, unpack2(rw[i], T()));
+                  w[i] = pack2(a.x, a.y, T());
+                }
               }
             }
+            *at = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
+        fence_proxy_async_smem();
+        __syncwarp();
 #pragma unroll
-        for (int v = 0; v < 8; ++v)
-          *reinterpret_cast<uint4*>(buf + swz(lane, v * 16)) =
-              make_uint4(w[4 * v], w[4 * v + 1], w[4 * v + 2], w[4 * v + 3]);
-        if (p.out_tma && (cols - cb >= E || p.out_tail)) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            tma_store_2d(&tmOut, buf, n0 + cb, m0);
-            tma_store_commit();
+        for (int b = b0; b < (b0 + 2 < kBlocks ? b0 + 2 : kBlocks); ++b) {
+          const int cb = b * E;
+          if (cb >= cols) break;
+          const uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
+          if (p.out_tma && (cols - cb >= E || p.out_tail)) {
+            if (lane == 0) tma_store_2d(&tmOut, buf, n0 + cb, m0);
+          } else {
+            T* dst = O == Out8::Q8 ? reinterpret_cast<T*>(p.g.q) : static_cast<T*>(p.g.out);
+            const int64_t ld = O == Out8::Q8 ? p.g.ldq : p.g.ldo;
+            store_block(buf, dst + static_cast<int64_t>(m0) * ld + n0 + cb, ld, rows, cols - cb, lane);
           }
-        } else {
-          __syncwarp();
-          T* dst = O == Out8::Q8 ? reinterpret_cast<T*>(p.g.q) : static_cast<T*>(p.g.out);
-          const int64_t ld = O == Out8::Q8 ? p.g.ldq : p.g.ldo;
-          store_block(buf, dst + static_cast<int64_t>(m0) * ld + n0 + cb, ld, rows, cols - cb, lane);
-          __syncwarp();
         }
+        if (lane == 0) tma_store_commit();
+        __syncwarp();
       }
     }
     cp_async_wait<0>();

@@ -28,6 +28,13 @@ constexpr float kMinScale8 = 1.17549435e-38f;  // 2^-126
 // number and NaN above infinity, so an integer maximum keeps a NaN.
 __device__ __forceinline__ uint32_t mag_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
+// max(a, |b|, |c|) for a >= 0; NaN if one of them is.
+__device__ __forceinline__ float max_mag3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 struct Scale8 {
   float s, inv;
 };

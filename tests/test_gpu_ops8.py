@@ -11,6 +11,8 @@ Bounds, derived from the arithmetic (u = 2^-24, half an ulp of fp32):
   each within 2u (an adder that truncates) of the sum of magnitudes; the product
   of the two scales, the scaling and the running total add 4u per block.  So
   |error| <= (128 + 2 * blocks + 8) * 2u * S with S = sum |a||w| in true values.
+  The running total starts from the bias: its magnitude joins every addition's,
+  so blocks * u * |bias| more.
 * gelu' is at most 1.13; the erf itself is within 2^-20.
 """
 import math
@@ -271,11 +273,12 @@ def test_gemm8(lb, m, n, k):
         want, lim = h, tol
         if with_bias:
             want = want + bias.double()
+            lim = lim + -(-k // 128) * U * bias.double().abs()
         if with_resid:
             want = want + resid.double()
         # two fp32 additions, then the rounding to the output's type (fp16: subnormal step 2^-25)
         size = tol + h.abs() + (bias.double().abs() if with_bias else 0) + (resid.double().abs() if with_resid else 0)
-        lim = tol + 2 * U * size + (want.abs() + tol) * torch.finfo(dt).eps / 2 + (2.0 ** -25 if kind == "f16" else 0)
+        lim = lim + 2 * U * size + (want.abs() + tol) * torch.finfo(dt).eps / 2 + (2.0 ** -25 if kind == "f16" else 0)
         err = (out.double() - want).abs()
         assert (err <= lim).all(), (kind, float((err / lim).max()))
         assert (buf[m] == 5.0).all() and (buf[:, n:] == 5.0).all()
@@ -290,7 +293,7 @@ def test_gemm8_gelu_quant8(lb, m, n, k, with_bias):
     h, tol = product(a64, w64, k)
     if with_bias:
         h = h + bias.double()
-        tol = tol + U * (h.abs() + tol)
+        tol = tol + U * (h.abs() + tol) + -(-k // 128) * U * bias.double().abs()
     g = 0.5 * h * torch.special.erfc(-h / math.sqrt(2.0))
     tol_g = 1.13 * tol + h.abs() * 2.0 ** -20
     q, s, buf = out8(m, n, pitch=n + 5)
@@ -407,7 +410,8 @@ def test_feed_forward_in_8_bits(lb, rows):
     g8 = b["g8"].double() * expand(b["g8s"].double(), rows, 1024, 1)
     h, tol = product(g8, w2, 1024)
     want = h + b["b2"].double() + y
-    assert ((b["y"].double() - want).abs() <= tol + 4 * U * (h.abs() + b["b2"].double().abs() + y.abs() + tol)).all()
+    assert ((b["y"].double() - want).abs() <= tol + 8 * U * b["b2"].double().abs()  # 8 blocks of K = 1024
+            + 4 * U * (h.abs() + b["b2"].double().abs() + y.abs() + tol)).all()
     # and the whole beside the fp16 feed-forward of the same weights: each branch value carries relative
     # errors of at most 2^-4 from four quantisations (norm, W1, gelu, W2); their root mean square is below
     # 2^-4 / sqrt(3) each, so the branch is within 4 * 2^-4 of its own size
