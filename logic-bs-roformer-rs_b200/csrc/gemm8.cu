@@ -25,8 +25,10 @@
 // never wait for a global load).
 #include <atomic>
 
+#include "cp_async.cuh"
 #include "fastdiv.cuh"
 #include "gelu8.cuh"
+#include "gemm8_few.cuh"
 #include "quant8.cuh"
 
 namespace lbrr {
@@ -91,24 +93,6 @@ __device__ __forceinline__ void tile8(const Params8& p, int idx, int& m0, int& n
   const int n = rows >= kGroup8 ? rem / kGroup8 : rem / rows;
   m0 = (gi * kGroup8 + rem - n * min(rows, kGroup8)) * (2 * kM8);
   n0 = n * kN8;
-}
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-// 4 bytes, or zero where `valid` is false.
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(valid ? 4 : 0)
-               : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// Arrive on the barrier (one of its counted arrivals) once this thread's copies so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Byte o of row r in a buffer of 32 rows of 128 bytes with the TMA 128-byte swizzle.
@@ -586,7 +570,7 @@ static cudaError_t launch8(const CUtensorMap& ta, const CUtensorMap& tw, const C
   return cudaGetLastError();
 }
 
-cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
+static cudaError_t gemm8_tiled(const Gemm8& g, int* status, cudaStream_t st) {
   CUtensorMap ta, tw, to;
   Params8 p;
   p.g = g;
@@ -614,6 +598,35 @@ cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
     case Elem::BF16: return launch8<Out8::BF16>(ta, tw, to, p, status, st);
   }
   return cudaErrorInvalidValue;
+}
+
+static cudaError_t gemm8_few(const Gemm8& g, int* status, cudaStream_t st) {
+  FewParams p;
+  p.g = g;
+  p.kb = (g.k + 127) / 128;
+  p.kind = g.out ? static_cast<int>(g.out_type) : 3;
+  const size_t size = !g.out ? 1 : g.out_type == Elem::F32 ? 4 : 2;
+  auto fours = [&](const void* ptr, int64_t ld, size_t sz) {  // 4 values at once from any multiple of 4 columns
+    return reinterpret_cast<uintptr_t>(ptr) % (4 * sz) == 0 && ld % 4 == 0;
+  };
+  p.vec = fours(g.out ? g.out : g.q, g.out ? g.ldo : g.ldq, size) && (!g.resid || fours(g.resid, g.ldr, size)) &&
+          (!g.bias || fours(g.bias, 0, 4));
+  const int nt = g.m <= 16 ? 16 : g.m <= 32 ? 32 : 64;
+  const int64_t tiles = static_cast<int64_t>((g.n + 127) / 128) * ((g.m + nt - 1) / nt);
+  // as many CTAs per tile as two per SM allow, each with a K-block at least
+  p.lg = 0;
+  while ((1 << p.lg) < kFewMaxSplit && (tiles << (p.lg + 1)) <= 2 * 148 && (2 << p.lg) <= p.kb) ++p.lg;
+  p.split = 1 << p.lg;
+  return nt == 16 ? launch_few<16>(p, status, st)
+                  : nt == 32 ? launch_few<32>(p, status, st) : launch_few<64>(p, status, st);
+}
+
+// Few rows of A, or so few 128 x 64 tiles that each SM has at most one, go to the kernel that splits K; measured
+// (bf16 out): 62 x 1536 x 256 5.1 us (tiled 6.3), 256 x 4096 x 4096 15.7 (18.4), 512 x 2048 x 2048 10.7 (12.2),
+// against 512 x 4096 x 4096 24.5 (18.9), 1024 x 2048 x 2048 15.4 (12.7), 2294 x 1536 x 256 10.2 (7.1).
+cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
+  const int64_t tiles = static_cast<int64_t>((g.m + 63) / 64) * ((g.n + 127) / 128);
+  return g.m <= 64 || tiles <= 148 ? gemm8_few(g, status, st) : gemm8_tiled(g, status, st);
 }
 
 }  // namespace lbrr
