@@ -4,7 +4,7 @@
 //
 // A block with largest magnitude t is held as q = e4m3(v / s), s = t / 448
 // (448: the largest finite e4m3 value).  Two roundings are choices: v / s is
-// computed as v * (1 / s) (within 1.5 ulp of 32 bits, far below e4m3's half
+// computed as v * (1 / s) (within 2 ulp of 32 bits, far below e4m3's half
 // step of 2^-4), and q is rounded to nearest even with saturation, so the
 // block's largest value, which may land an ulp above 448, stays 448.  s is at
 // least 2^-126, so 1 / s is finite and a block of zeros is held as zeros.  A
@@ -44,8 +44,11 @@ __device__ __forceinline__ Scale8 scale8(uint32_t top) {
   if (top >= 0x7f800000u) {
     r.s = r.inv = __uint_as_float(0x7fffffffu);
   } else {
-    r.s = fmaxf(__fdiv_rn(__uint_as_float(top), kE4m3Max), kMinScale8);
-    r.inv = __frcp_rn(r.s);
+    // t / 448, correctly rounded: the product with 1 / 448, corrected once by its remainder (exact in an FMA)
+    const float t = __uint_as_float(top), c = 1.0f / kE4m3Max;
+    const float q = t * c;
+    r.s = fmaxf(fmaf(fmaf(-q, kE4m3Max, t), c, q), kMinScale8);
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));  // within 1 ulp
   }
   return r;
 }
