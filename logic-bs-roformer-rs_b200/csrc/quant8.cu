@@ -3,6 +3,8 @@
 // addition and an 8-bit output.  Both are one pass over their data (every
 // value is read once, held in registers while its block's or row's statistics
 // form, and written once), so HBM bounds them.
+#include <cmath>
+
 #include "quant8.cuh"
 
 namespace lbrr {
@@ -32,14 +34,15 @@ __global__ void __launch_bounds__(kWarps8 * 32)
       for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
     }
   }
-  const int kb = blockIdx.y * 2 + (lane >> 4);
+  uint32_t top[kRows8];
 #pragma unroll
-  for (int i = 0; i < kRows8; ++i) {
-    const Scale8 s = scale8(half_warp_max(top_of(v[i])));
-    if (r0 + i >= rows) break;
-    store_codes<VEC>(q + static_cast<int64_t>(r0 + i) * ldq, c0, cols, lane, v[i], s.inv);
-    if ((lane & 15) == 0 && kb * kBlock8 < cols) scales[kb * lds + r0 + i] = s.s;
-  }
+  for (int i = 0; i < kRows8; ++i) top[i] = top_of(v[i]);
+  const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
+#pragma unroll
+  for (int i = 0; i < kRows8; ++i)
+    if (r0 + i < rows) store_codes<VEC>(q + static_cast<int64_t>(r0 + i) * ldq, c0, cols, lane, v[i], sc.inv[i]);
+  const int kb = blockIdx.y * 2 + (lane >> 4);
+  if (sc.writer && r0 + sc.own_block < rows && kb * kBlock8 < cols) scales[kb * lds + r0 + sc.own_block] = sc.own;
 }
 
 // Blocks of 128 x 128: one CTA per block, 32 values per thread.
@@ -155,7 +158,8 @@ template <class TX, class TR, int C, bool VEC>
 __global__ void __launch_bounds__(C >= 4 ? 1024 : 512)
     add_norm_quant_kernel(const TX* x, int64_t ldx, const TR* resid, int64_t ldr, const float* __restrict__ gamma,
                           float eps, TR* y, int64_t ldy, uint8_t* __restrict__ q, int64_t ldq,
-                          float* __restrict__ scales, int64_t lds, int rows, int cols, int warps) {
+                          float* __restrict__ scales, int64_t lds, int rows, int cols, int warps, float inv_cols,
+                          float most) {
   __shared__ RowSum sh;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_cta = warps == 1 ? blockDim.x >> 5 : 1;
@@ -178,13 +182,15 @@ __global__ void __launch_bounds__(C >= 4 ? 1024 : 512)
       for (int i = 0; i < C; ++i) store_cols<VEC>(y + row * ldy, (wr + i * warps) * 256, cols, lane, v[i]);
     }
   }
-  float ss = 0.0f;
+  float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
   for (int i = 0; i < C; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = fmaf(v[i][j], v[i][j], ss);
-  ss = row_sum(ss, sh.part, warps, wr, lane);
-  const float n = static_cast<float>(cols);
+    for (int j = 0; j < 8; j += 2) {
+      const float2 u = make_float2(v[i][j], v[i][j + 1]);
+      sq = __ffma2_rn(u, u, sq);
+    }
+  const float ss = row_sum(sq.x + sq.y, sh.part, warps, wr, lane);
   float inv;
   if (ss == __int_as_float(0x7f800000)) {  // the same for every thread of the row
     uint32_t top = 0;
@@ -204,25 +210,31 @@ __global__ void __launch_bounds__(C >= 4 ? 1024 : 512)
           t = fmaf(v[i][j], v[i][j], t);
         }
       t = row_sum(t, sh.part, warps, wr, lane);
-      inv = 1.0f / sqrtf(t / n);  // eps and the floor are below rounding here
+      inv = rsqrtf(t * inv_cols);  // eps and the floor are below rounding here
     }
   } else {
-    inv = 1.0f / fmaxf(sqrtf(ss / n + eps), 1e-12f / sqrtf(n));
-    if (ss != ss) inv = ss;  // fmaxf drops a NaN
+    inv = fminf(rsqrtf(ss * inv_cols + eps), most);  // rsqrtf: within 2 ulp
+    if (ss != ss) inv = ss;  // fminf drops a NaN
   }
+  uint32_t tops[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int c0 = (wr + i * warps) * 256;
-    if (c0 >= cols) break;
     float g[8];
-    load_cols<VEC>(gamma, c0, cols, lane, g);
+    load_cols<VEC>(gamma, (wr + i * warps) * 256, cols, lane, g);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[i][j] = (v[i][j] * inv) * g[j];
-    const Scale8 s = scale8(half_warp_max(top_of(v[i])));
-    store_codes<VEC>(q + row * ldq, c0, cols, lane, v[i], s.inv);
-    const int kb = (c0 >> 7) + (lane >> 4);
-    if ((lane & 15) == 0 && kb * kBlock8 < cols) scales[kb * lds + row] = s.s;
+    for (int j = 0; j < 8; j += 2) {
+      const float2 u = __fmul2_rn(__fmul2_rn(make_float2(v[i][j], v[i][j + 1]), make_float2(inv, inv)),
+                                  make_float2(g[j], g[j + 1]));
+      v[i][j] = u.x;
+      v[i][j + 1] = u.y;
+    }
+    tops[i] = top_of(v[i]);
   }
+  const Scales8<C> sc = half_warp_scales<C>(tops, lane);
+#pragma unroll
+  for (int i = 0; i < C; ++i) store_codes<VEC>(q + row * ldq, (wr + i * warps) * 256, cols, lane, v[i], sc.inv[i]);
+  const int kb = (wr + sc.own_block * warps) * 2 + (lane >> 4);
+  if (sc.writer && kb * kBlock8 < cols) scales[kb * lds + row] = sc.own;
 }
 
 template <class TX, class TR>
@@ -244,13 +256,15 @@ static cudaError_t add_norm_quant8_t(const AddNorm8& a, cudaStream_t st) {
     warps = (chunks + c - 1) / c;
     threads = warps * 32;
   }
+  const float inv_cols = 1.0f / static_cast<float>(a.cols);
+  const float most = static_cast<float>(std::sqrt(static_cast<double>(a.cols)) * 1e12);  // 1 / the norm's floor
   const int per_cta = warps == 1 ? threads / 32 : 1;
   const int grid = (a.rows + per_cta - 1) / per_cta;
   count_launch();
 #define LBRR_LAUNCH(CC)                                                                                            \
   (vec ? add_norm_quant_kernel<TX, TR, CC, true> : add_norm_quant_kernel<TX, TR, CC, false>)<<<grid, threads, 0,   \
                                                                                                st>>>(             \
-      x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds, a.rows, a.cols, warps)
+      x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds, a.rows, a.cols, warps, inv_cols, most)
   switch (c) {
     case 1: LBRR_LAUNCH(1); break;
     case 2: LBRR_LAUNCH(2); break;

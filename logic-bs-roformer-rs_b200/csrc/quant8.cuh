@@ -157,29 +157,69 @@ __device__ __forceinline__ void store_cols(T* row, int c0, int cols, int lane, c
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int lane, const float (&v)[8],
                                             float inv) {
-  const uint32_t lo = e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  const uint32_t hi = e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv);
+  const float2 f = make_float2(inv, inv);
+  const float2 a = __fmul2_rn(make_float2(v[0], v[1]), f), b = __fmul2_rn(make_float2(v[2], v[3]), f);
+  const float2 c = __fmul2_rn(make_float2(v[4], v[5]), f), d = __fmul2_rn(make_float2(v[6], v[7]), f);
+  const uint32_t lo = e4m3x4(a.x, a.y, b.x, b.y), hi = e4m3x4(c.x, c.y, d.x, d.y);
   if (VEC && c0 + lane * 8 + 8 <= cols) {
     *reinterpret_cast<uint2*>(row + c0 + lane * 8) = make_uint2(lo, hi);
     return;
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const int c = c0 + lane_col<VEC>(lane, j);
-    if (c < cols) row[c] = static_cast<uint8_t>((j < 4 ? lo >> (8 * j) : hi >> (8 * (j - 4))) & 0xffu);
+    const int at = c0 + lane_col<VEC>(lane, j);
+    if (at < cols) row[at] = static_cast<uint8_t>((j < 4 ? lo >> (8 * j) : hi >> (8 * (j - 4))) & 0xffu);
   }
 }
+// Largest magnitude of eight values, as bits (NaN above all).
 __device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, mag_bits(v[j]));
-  return m;
+  const float a = max_mag3(0.0f, v[0], v[1]), b = max_mag3(0.0f, v[4], v[5]);
+  return __float_as_uint(max_mag3(max_mag3(a, v[2], v[3]), max_mag3(b, v[6], v[7]), 0.0f));
 }
-// Maximum over the 16 lanes that share a block.
-__device__ __forceinline__ uint32_t half_warp_max(uint32_t m) {
+
+// The scales of R blocks (1, 2 or 4) that 16 lanes hold together: from every
+// lane's own maxima, each block's inverse scale in every lane, and its scale in
+// lane `own_block`'s lanes.  The exchange halves the number of blocks a lane
+// follows until it has one, so R blocks take R + 3 shuffles (and R to hand the
+// inverses back), not 4 R, and one scale per lane is computed, not R.
+template <int R>
+struct Scales8 {
+  float inv[R];
+  float own;       // the scale of block own_block
+  int own_block;
+  bool writer;     // one lane per block
+};
+template <int R>
+__device__ __forceinline__ Scales8<R> half_warp_scales(const uint32_t (&top)[R], int lane) {
+  static_assert(R == 1 || R == 2 || R == 4, "blocks");
+  constexpr unsigned all = 0xffffffffu;
+  uint32_t k;
+  const bool b3 = lane & 8, b2 = lane & 4;
+  Scales8<R> r;
+  if constexpr (R == 4) {
+    const uint32_t x = max(b3 ? top[2] : top[0], __shfl_xor_sync(all, b3 ? top[0] : top[2], 8));
+    const uint32_t y = max(b3 ? top[3] : top[1], __shfl_xor_sync(all, b3 ? top[1] : top[3], 8));
+    k = max(b2 ? y : x, __shfl_xor_sync(all, b2 ? x : y, 4));
+    r.own_block = (lane >> 2) & 3;
+    r.writer = (lane & 3) == 0;
+  } else if constexpr (R == 2) {
+    k = max(b3 ? top[1] : top[0], __shfl_xor_sync(all, b3 ? top[0] : top[1], 8));
+    k = max(k, __shfl_xor_sync(all, k, 4));
+    r.own_block = (lane >> 3) & 1;
+    r.writer = (lane & 7) == 0;
+  } else {
+    k = max(top[0], __shfl_xor_sync(all, top[0], 8));
+    k = max(k, __shfl_xor_sync(all, k, 4));
+    r.own_block = 0;
+    r.writer = (lane & 15) == 0;
+  }
+  k = max(k, __shfl_xor_sync(all, k, 2));
+  k = max(k, __shfl_xor_sync(all, k, 1));
+  const Scale8 s = scale8(k);
+  r.own = s.s;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-  return m;
+  for (int i = 0; i < R; ++i) r.inv[i] = R == 1 ? s.inv : __shfl_sync(all, s.inv, (lane & 16) | (i * (16 / R)));
+  return r;
 }
 
 }  // namespace lbrr
