@@ -3,6 +3,7 @@
 // addition and an 8-bit output.  Both are one pass over their data (every
 // value is read once, held in registers while its block's or row's statistics
 // form, and written once), so HBM bounds them.
+#include <algorithm>
 #include <cmath>
 
 #include "quant8.cuh"
@@ -11,38 +12,51 @@ namespace lbrr {
 
 // ---------------------------------------------------------------------------
 // v -> (q, scales), blocks of 1 x 128.  A warp takes kRows8 rows of 256
-// columns (16 lanes per block), all loads issued before the first use; eight
-// warps cover 32 rows, so the scales of a block column leave as whole sectors.
+// columns (16 lanes per block) at a time and has the next ones' loads in flight
+// meanwhile; eight warps cover 32 rows, so the scales of a block column leave
+// as whole sectors.
 // ---------------------------------------------------------------------------
 constexpr int kRows8 = 4;
 constexpr int kWarps8 = 8;
+constexpr int kBlocksPerSm8 = 4;
 
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kWarps8 * 32)
+__global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
     quant_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
                       float* __restrict__ scales, int64_t lds) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int r0 = (blockIdx.x * kWarps8 + warp) * kRows8;
   const int c0 = blockIdx.y * 2 * kBlock8;
-  float v[kRows8][8];
+  Raw8<T> next[kRows8];
+  auto fetch = [&](int r0) {
 #pragma unroll
-  for (int i = 0; i < kRows8; ++i) {
-    if (r0 + i < rows) {
-      load_cols<VEC>(x + static_cast<int64_t>(r0 + i) * ldx, c0, cols, lane, v[i]);
-    } else {
+    for (int i = 0; i < kRows8; ++i)
+      if (r0 + i < rows) load_raw<VEC>(x + static_cast<int64_t>(r0 + i) * ldx, c0, cols, lane, next[i]);
+  };
+  const int step = gridDim.x * kWarps8 * kRows8;
+  int r0 = (blockIdx.x * kWarps8 + warp) * kRows8;
+  fetch(r0);
+  for (; r0 < rows; r0 += step) {
+    float v[kRows8][8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    for (int i = 0; i < kRows8; ++i) {
+      if (r0 + i < rows) {
+        next[i].get(v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+      }
     }
+    fetch(r0 + step);
+    uint32_t top[kRows8];
+#pragma unroll
+    for (int i = 0; i < kRows8; ++i) top[i] = top_of(v[i]);
+    const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
+#pragma unroll
+    for (int i = 0; i < kRows8; ++i)
+      if (r0 + i < rows) store_codes<VEC>(q + static_cast<int64_t>(r0 + i) * ldq, c0, cols, lane, v[i], sc.inv[i]);
+    const int kb = blockIdx.y * 2 + (lane >> 4);
+    if (sc.writer && r0 + sc.own_block < rows && kb * kBlock8 < cols) scales[kb * lds + r0 + sc.own_block] = sc.own;
   }
-  uint32_t top[kRows8];
-#pragma unroll
-  for (int i = 0; i < kRows8; ++i) top[i] = top_of(v[i]);
-  const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
-#pragma unroll
-  for (int i = 0; i < kRows8; ++i)
-    if (r0 + i < rows) store_codes<VEC>(q + static_cast<int64_t>(r0 + i) * ldq, c0, cols, lane, v[i], sc.inv[i]);
-  const int kb = blockIdx.y * 2 + (lane >> 4);
-  if (sc.writer && r0 + sc.own_block < rows && kb * kBlock8 < cols) scales[kb * lds + r0 + sc.own_block] = sc.own;
 }
 
 // Blocks of 128 x 128: one CTA per block, 32 values per thread.
@@ -96,7 +110,10 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
   const bool vec = rows_aligned(x, ldx, sizeof(T), 16) && rows_aligned(q, ldq, 1, 8);
   count_launch();
   if (block_rows == 1) {
-    const dim3 grid((rows + kWarps8 * kRows8 - 1) / (kWarps8 * kRows8), (cols + 2 * kBlock8 - 1) / (2 * kBlock8));
+    const int groups = (rows + kWarps8 * kRows8 - 1) / (kWarps8 * kRows8);
+    const int chunks = (cols + 2 * kBlock8 - 1) / (2 * kBlock8);
+    const int resident = std::max(1, kBlocksPerSm8 * 148 / chunks);  // blocks per column chunk that run at one time
+    const dim3 grid(std::min(groups, resident), chunks);
     auto k = vec ? quant_rows_kernel<T, true> : quant_rows_kernel<T, false>;
     k<<<grid, kWarps8 * 32, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds);
   } else {
@@ -122,7 +139,7 @@ cudaError_t quant8(const void* x, Elem type, int64_t ldx, int rows, int cols, in
 // 1e-12 / sqrt(cols)); n -> (q, scales) by 1 x 128.
 //
 // With eps = 0 this is the trunk's norm, y * sqrt(cols) / max(|y|, 1e-12).  A
-// row belongs to `warps` warps (one warp up to 1024 columns, so those rows need
+// row belongs to `warps` warps (one warp up to 512 columns, so those rows need
 // no block barrier), each holding C chunks of 256 columns in registers; the
 // sum of squares is 32-bit.  Where it overflows (rows beyond 1e17) the row is
 // scaled by the power of two that brings its largest value near 2^32 and
@@ -154,8 +171,8 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, uint32_t* part, int warp
   return t;
 }
 
-template <class TX, class TR, int C, bool VEC>
-__global__ void __launch_bounds__(C >= 4 ? 1024 : 512)
+template <class TX, class TR, int C, bool VEC, bool LOOP, int THREADS>
+__global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1)
     add_norm_quant_kernel(const TX* x, int64_t ldx, const TR* resid, int64_t ldr, const float* __restrict__ gamma,
                           float eps, TR* y, int64_t ldy, uint8_t* __restrict__ q, int64_t ldq,
                           float* __restrict__ scales, int64_t lds, int rows, int cols, int warps, float inv_cols,
@@ -164,77 +181,94 @@ __global__ void __launch_bounds__(C >= 4 ? 1024 : 512)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per_cta = warps == 1 ? blockDim.x >> 5 : 1;
   const int wr = warps == 1 ? 0 : warp;  // this warp's place in its row
-  const int row = blockIdx.x * per_cta + (warps == 1 ? warp : 0);
-  if (row >= rows) return;  // whole warps, and whole blocks where a row spans a block
-  float v[C][8];
-#pragma unroll
-  for (int i = 0; i < C; ++i) load_cols<VEC>(x + row * ldx, (wr + i * warps) * 256, cols, lane, v[i]);
-  if (resid) {
+  const int step = gridDim.x * per_cta;
+  Raw8<TX> nx[C];
+  Raw8<TR> nr[C];
+  auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      float r[8];
-      load_cols<VEC>(resid + row * ldr, (wr + i * warps) * 256, cols, lane, r);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+      load_raw<VEC>(x + r * ldx, (wr + i * warps) * 256, cols, lane, nx[i]);
+      if (resid) load_raw<VEC>(resid + r * ldr, (wr + i * warps) * 256, cols, lane, nr[i]);
     }
-    if (y) {
+  };
+  int64_t row = blockIdx.x * per_cta + (warps == 1 ? warp : 0);
+  if (row >= rows) return;  // whole warps, and whole blocks where a row spans a block
+  fetch(row);
+  for (;; row += step) {
+    float v[C][8];
 #pragma unroll
-      for (int i = 0; i < C; ++i) store_cols<VEC>(y + row * ldy, (wr + i * warps) * 256, cols, lane, v[i]);
+    for (int i = 0; i < C; ++i) nx[i].get(v[i]);
+    if (resid) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float r[8];
+        nr[i].get(r);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] += r[j];
+      }
+      if (LOOP && row + step < rows) fetch(row + step);
+      if (y) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) store_cols<VEC>(y + row * ldy, (wr + i * warps) * 256, cols, lane, v[i]);
+      }
+    } else if (LOOP && row + step < rows) {
+      fetch(row + step);
     }
-  }
-  float2 sq = make_float2(0.0f, 0.0f);
+    float2 sq = make_float2(0.0f, 0.0f);
 #pragma unroll
-  for (int i = 0; i < C; ++i)
+    for (int i = 0; i < C; ++i)
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float2 u = make_float2(v[i][j], v[i][j + 1]);
-      sq = __ffma2_rn(u, u, sq);
-    }
-  const float ss = row_sum(sq.x + sq.y, sh.part, warps, wr, lane);
-  float inv;
-  if (ss == __int_as_float(0x7f800000)) {  // the same for every thread of the row
-    uint32_t top = 0;
+      for (int j = 0; j < 8; j += 2) {
+        const float2 u = make_float2(v[i][j], v[i][j + 1]);
+        sq = __ffma2_rn(u, u, sq);
+      }
+    const float ss = row_sum(sq.x + sq.y, sh.part, warps, wr, lane);
+    float inv;
+    if (ss == __int_as_float(0x7f800000)) {  // the same for every thread of the row
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < C; ++i) top = max(top, top_of(v[i]));
-    top = row_max(top, sh.top, warps, wr, lane);
-    if (top >= 0x7f800000u) {
-      inv = 0.0f;  // an infinity in the row: its finite values are 0 beside it, itself NaN
+      for (int i = 0; i < C; ++i) top = max(top, top_of(v[i]));
+      top = row_max(top, sh.top, warps, wr, lane);
+      if (top >= 0x7f800000u) {
+        inv = 0.0f;  // an infinity in the row: its finite values are 0 beside it, itself NaN
+      } else {
+        const float down = __uint_as_float((286u - (top >> 23)) << 23);  // brings the largest value to [2^32, 2^33)
+        float t = 0.0f;
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            v[i][j] *= down;
+            t = fmaf(v[i][j], v[i][j], t);
+          }
+        t = row_sum(t, sh.part, warps, wr, lane);
+        inv = rsqrtf(t * inv_cols);  // eps and the floor are below rounding here
+      }
     } else {
-      const float down = __uint_as_float((286u - (top >> 23)) << 23);  // brings the largest value to [2^32, 2^33)
-      float t = 0.0f;
-#pragma unroll
-      for (int i = 0; i < C; ++i)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          v[i][j] *= down;
-          t = fmaf(v[i][j], v[i][j], t);
-        }
-      t = row_sum(t, sh.part, warps, wr, lane);
-      inv = rsqrtf(t * inv_cols);  // eps and the floor are below rounding here
+      inv = fminf(rsqrtf(ss * inv_cols + eps), most);  // rsqrtf: within 2 ulp
+      if (ss != ss) inv = ss;  // fminf drops a NaN
     }
-  } else {
-    inv = fminf(rsqrtf(ss * inv_cols + eps), most);  // rsqrtf: within 2 ulp
-    if (ss != ss) inv = ss;  // fminf drops a NaN
-  }
-  uint32_t tops[C];
+    uint32_t tops[C];
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    float g[8];
-    load_cols<VEC>(gamma, (wr + i * warps) * 256, cols, lane, g);
+    for (int i = 0; i < C; ++i) {
+      float g[8];
+      load_cols<VEC>(gamma, (wr + i * warps) * 256, cols, lane, g);
 #pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float2 u = __fmul2_rn(__fmul2_rn(make_float2(v[i][j], v[i][j + 1]), make_float2(inv, inv)),
-                                  make_float2(g[j], g[j + 1]));
-      v[i][j] = u.x;
-      v[i][j + 1] = u.y;
+      for (int j = 0; j < 8; j += 2) {
+        const float2 u = __fmul2_rn(__fmul2_rn(make_float2(v[i][j], v[i][j + 1]), make_float2(inv, inv)),
+                                    make_float2(g[j], g[j + 1]));
+        v[i][j] = u.x;
+        v[i][j + 1] = u.y;
+      }
+      tops[i] = top_of(v[i]);
     }
-    tops[i] = top_of(v[i]);
-  }
-  const Scales8<C> sc = half_warp_scales<C>(tops, lane);
+    const Scales8<C> sc = half_warp_scales<C>(tops, lane);
 #pragma unroll
-  for (int i = 0; i < C; ++i) store_codes<VEC>(q + row * ldq, (wr + i * warps) * 256, cols, lane, v[i], sc.inv[i]);
-  const int kb = (wr + sc.own_block * warps) * 2 + (lane >> 4);
-  if (sc.writer && kb * kBlock8 < cols) scales[kb * lds + row] = sc.own;
+    for (int i = 0; i < C; ++i) store_codes<VEC>(q + row * ldq, (wr + i * warps) * 256, cols, lane, v[i], sc.inv[i]);
+    const int kb = (wr + sc.own_block * warps) * 2 + (lane >> 4);
+    if (sc.writer && kb * kBlock8 < cols) scales[kb * lds + row] = sc.own;
+    if (!LOOP || row + step >= rows) break;
+  }
 }
 
 template <class TX, class TR>
@@ -246,29 +280,30 @@ static cudaError_t add_norm_quant8_t(const AddNorm8& a, cudaStream_t st) {
                    (!y || rows_aligned(y, a.ldy, sizeof(TR), 16)) && rows_aligned(a.q, a.ldq, 1, 8) &&
                    rows_aligned(a.gamma, 0, 4, 16);
   const int chunks = (a.cols + 255) / 256;
-  int c, warps, threads;
-  if (chunks <= 4) {  // one warp per row
-    c = chunks <= 1 ? 1 : chunks <= 2 ? 2 : 4;
-    warps = 1;
-    threads = 128;
-  } else {  // one block per row
-    c = chunks <= 32 ? 2 : 4;
-    warps = (chunks + c - 1) / c;
-    threads = warps * 32;
-  }
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   const float most = static_cast<float>(std::sqrt(static_cast<double>(a.cols)) * 1e12);  // 1 / the norm's floor
-  const int per_cta = warps == 1 ? threads / 32 : 1;
-  const int grid = (a.rows + per_cta - 1) / per_cta;
   count_launch();
-#define LBRR_LAUNCH(CC)                                                                                            \
-  (vec ? add_norm_quant_kernel<TX, TR, CC, true> : add_norm_quant_kernel<TX, TR, CC, false>)<<<grid, threads, 0,   \
-                                                                                               st>>>(             \
-      x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds, a.rows, a.cols, warps, inv_cols, most)
-  switch (c) {
-    case 1: LBRR_LAUNCH(1); break;
-    case 2: LBRR_LAUNCH(2); break;
-    default: LBRR_LAUNCH(4); break;
+#define LBRR_LAUNCH(CC, LOOP, MAX)                                                                                \
+  (vec ? add_norm_quant_kernel<TX, TR, CC, true, LOOP, MAX> : add_norm_quant_kernel<TX, TR, CC, false, LOOP, MAX>) \
+      <<<grid, threads, 0, st>>>(x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds,   \
+                                 a.rows, a.cols, warps, inv_cols, most)
+  if (chunks <= 2) {  // a warp per row
+    constexpr int warps = 1, threads = 128;
+    const int grid = (a.rows + 3) / 4;
+    if (chunks == 1)
+      LBRR_LAUNCH(1, false, threads);
+    else
+      LBRR_LAUNCH(2, false, threads);
+  } else if (chunks <= 64) {  // a block per row, the next row's loads in flight; as many blocks as run at one time
+    const int warps = (chunks + 1) / 2, threads = warps * 32;
+    const int grid = std::min(a.rows, 148 * (1024 / threads));
+    if (threads <= 512)
+      LBRR_LAUNCH(2, true, 512);
+    else
+      LBRR_LAUNCH(2, true, 1024);
+  } else {  // rows whose registers leave no room for the next one's
+    const int warps = (chunks + 3) / 4, threads = warps * 32, grid = a.rows;
+    LBRR_LAUNCH(4, false, 1024);
   }
 #undef LBRR_LAUNCH
   return cudaGetLastError();

@@ -130,6 +130,45 @@ template <bool VEC>
 __device__ __forceinline__ int lane_col(int lane, int j) {
   return VEC ? lane * 8 + j : (lane >> 4) * kBlock8 + (lane & 15) + 16 * j;
 }
+// Eight values as they are in memory, for loads that are issued well before their use.
+template <class T>
+struct Raw8 {
+  union {
+    uint4 w[sizeof(T) / 2];
+    T t[8];
+  };
+  __device__ __forceinline__ Raw8() {}
+  __device__ __forceinline__ void get(float (&v)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        v[4 * j] = __uint_as_float(w[j].x), v[4 * j + 1] = __uint_as_float(w[j].y);
+        v[4 * j + 2] = __uint_as_float(w[j].z), v[4 * j + 3] = __uint_as_float(w[j].w);
+      }
+    } else {
+      const float2 f0 = unpack2(w[0].x, T()), f1 = unpack2(w[0].y, T()), f2 = unpack2(w[0].z, T()),
+                   f3 = unpack2(w[0].w, T());
+      v[0] = f0.x, v[1] = f0.y, v[2] = f1.x, v[3] = f1.y;
+      v[4] = f2.x, v[5] = f2.y, v[6] = f3.x, v[7] = f3.y;
+    }
+  }
+};
+template <bool VEC, class T>
+__device__ __forceinline__ void load_raw(const T* row, int c0, int cols, int lane, Raw8<T>& r) {
+  if (VEC && c0 + lane * 8 + 8 <= cols) {
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j)
+      r.w[j] = reinterpret_cast<const uint4*>(row + c0 + lane * 8)[j];
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) r.w[j] = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const int c = c0 + lane_col<VEC>(lane, j);
+    if (c < cols) r.t[j] = row[c];
+  }
+}
 template <bool VEC, class T>
 __device__ __forceinline__ void load_cols(const T* row, int c0, int cols, int lane, float (&v)[8]) {
   if (VEC && c0 + lane * 8 + 8 <= cols) {
