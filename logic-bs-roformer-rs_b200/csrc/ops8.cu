@@ -70,7 +70,7 @@ extern "C" int lbrr_op_quant8(const void* x, int32_t x_type, int64_t ldx, int64_
   if (block_rows != 1 && block_rows != 128) return bad(op, "block_rows must be 1 or 128");
   if (rows < 0 || rows > kMaxRows || cols <= 0 || cols > kMaxCols) return bad(op, "bad rows or cols");
   if (rows == 0) return LBRR_OK;
-  if (block_rows == 128 && blocks(rows) > 65535) return bad(op, "128-row blocks take at most 8388480 rows");
+  if (block_rows == 128 && blocks(rows) * blocks(cols) > (1ll << 30)) return bad(op, "more than 2^30 blocks");
   if (!ok_matrix(x, ldx, cols, size_of(x_type))) return bad(op, "bad x");
   if (!ok_matrix(q, ldq, cols, 1)) return bad(op, "bad q");
   if (!ok_matrix(scales, lds, block_rows == 1 ? rows : blocks(rows), 4)) return bad(op, "bad scales");

@@ -20,83 +20,105 @@ constexpr int kRows8 = 4;
 constexpr int kWarps8 = 8;
 constexpr int kBlocksPerSm8 = 4;
 
-template <class T, bool VEC>
+// NARROW (up to 128 columns): the two halves of a warp take rows of their own.
+template <class T, bool VEC, bool NARROW>
 __global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
     quant_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
                       float* __restrict__ scales, int64_t lds) {
+  constexpr int kPerWarp = NARROW ? 2 * kRows8 : kRows8;  // rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int half = lane >> 4, at = NARROW ? lane & 15 : lane;  // `at`: this lane's columns
   const int c0 = blockIdx.y * 2 * kBlock8;
+  auto row_of = [&](int r0, int i) { return NARROW ? r0 + 2 * i + half : r0 + i; };
   Raw8<T> next[kRows8];
   auto fetch = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < kRows8; ++i)
-      if (r0 + i < rows) load_raw<VEC>(x + static_cast<int64_t>(r0 + i) * ldx, c0, cols, lane, next[i]);
+      if (row_of(r0, i) < rows)
+        load_raw<VEC>(x + static_cast<int64_t>(row_of(r0, i)) * ldx, c0, cols, at, next[i]);
   };
-  const int step = gridDim.x * kWarps8 * kRows8;
-  int r0 = (blockIdx.x * kWarps8 + warp) * kRows8;
+  const int step = gridDim.x * kWarps8 * kPerWarp;
+  int r0 = (blockIdx.x * kWarps8 + warp) * kPerWarp;
   fetch(r0);
   for (; r0 < rows; r0 += step) {
     float v[kRows8][8];
+    uint32_t top[kRows8];
 #pragma unroll
     for (int i = 0; i < kRows8; ++i) {
-      if (r0 + i < rows) {
+      if (row_of(r0, i) < rows) {
         next[i].get(v[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
       }
+      top[i] = top_of(v[i]);
     }
     fetch(r0 + step);
-    uint32_t top[kRows8];
-#pragma unroll
-    for (int i = 0; i < kRows8; ++i) top[i] = top_of(v[i]);
     const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
 #pragma unroll
     for (int i = 0; i < kRows8; ++i)
-      if (r0 + i < rows) store_codes<VEC>(q + static_cast<int64_t>(r0 + i) * ldq, c0, cols, lane, v[i], sc.inv[i]);
-    const int kb = blockIdx.y * 2 + (lane >> 4);
-    if (sc.writer && r0 + sc.own_block < rows && kb * kBlock8 < cols) scales[kb * lds + r0 + sc.own_block] = sc.own;
+      if (row_of(r0, i) < rows)
+        store_codes<VEC>(q + static_cast<int64_t>(row_of(r0, i)) * ldq, c0, cols, at, v[i], sc.inv[i]);
+    const int own = row_of(r0, sc.own_block), kb = NARROW ? 0 : blockIdx.y * 2 + half;
+    if (sc.writer && own < rows && kb * kBlock8 < cols) scales[kb * lds + own] = sc.own;
   }
 }
 
-// Blocks of 128 x 128: one CTA per block, 32 values per thread.
+// Blocks of 128 x 128: 32 values per thread.  16-bit inputs: two CTAs per SM
+// walk the blocks with the next one's loads in flight (71362 x 512: 33 -> 22 us);
+// 32-bit inputs leave no registers for that, so each block has its own CTA
+// (8192 x 8192: 51 us, 61 with the loop).  `blocks_x`: blocks side by side.
 constexpr int kTileThreads8 = 512;
 template <class T, bool VEC>
-__global__ void __launch_bounds__(kTileThreads8)
+__global__ void __launch_bounds__(kTileThreads8, 2)
     quant_tiles_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
-                       float* __restrict__ scales, int64_t lds) {
+                       float* __restrict__ scales, int64_t lds, int blocks_x, int blocks) {
   constexpr int kPer = kBlock8 * kBlock8 / kTileThreads8 / 8;  // row groups per thread
   constexpr int kStep = kTileThreads8 / 16;                    // rows per group
-  __shared__ uint32_t part[kTileThreads8 / 32];
+  __shared__ uint32_t part[2][kTileThreads8 / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int l16 = lane & 15;  // the 16 lanes of a row
-  const int r0 = blockIdx.y * kBlock8 + (threadIdx.x >> 4);
-  const int c0 = blockIdx.x * kBlock8;
-  float v[kPer][8];
-  uint32_t top = 0;
+  Raw8<T> next[kPer];
+  auto fetch = [&](int block) {
+    const int by = block / blocks_x, c0 = (block - by * blocks_x) * kBlock8;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int r = r0 + i * kStep;
-    if (r < rows) {
-      load_cols<VEC>(x + static_cast<int64_t>(r) * ldx, c0, cols, l16, v[i]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+    for (int i = 0; i < kPer; ++i) {
+      const int r = by * kBlock8 + (threadIdx.x >> 4) + i * kStep;
+      if (r < rows) load_raw<VEC>(x + static_cast<int64_t>(r) * ldx, c0, cols, l16, next[i]);
     }
-  }
+  };
+  constexpr bool kAhead = sizeof(T) == 2;
+  int block = blockIdx.x;
+  fetch(block);
+  for (int it = 0; block < blocks; block += gridDim.x, it ^= 1) {
+    const int by = block / blocks_x, bx = block - by * blocks_x;
+    const int r0 = by * kBlock8 + (threadIdx.x >> 4);
+    float v[kPer][8];
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) top = max(top, top_of(v[i]));
-  top = __reduce_max_sync(0xffffffffu, top);
-  if (lane == 0) part[warp] = top;
-  __syncthreads();
-  top = __reduce_max_sync(0xffffffffu, part[lane & (kTileThreads8 / 32 - 1)]);
-  const Scale8 s = scale8(top);
+    for (int i = 0; i < kPer; ++i) {
+      if (r0 + i * kStep < rows) {
+        next[i].get(v[i]);
+      } else {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int r = r0 + i * kStep;
-    if (r < rows) store_codes<VEC>(q + static_cast<int64_t>(r) * ldq, c0, cols, l16, v[i], s.inv);
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+      }
+      top = max(top, top_of(v[i]));
+    }
+    if (kAhead && block + static_cast<int>(gridDim.x) < blocks) fetch(block + gridDim.x);
+    top = __reduce_max_sync(0xffffffffu, top);
+    if (lane == 0) part[it][warp] = top;
+    __syncthreads();  // one per block: the next block writes the other half of `part`
+    top = __reduce_max_sync(0xffffffffu, part[it][lane & (kTileThreads8 / 32 - 1)]);
+    const Scale8 s = scale8(top);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int r = r0 + i * kStep;
+      if (r < rows) store_codes<VEC>(q + static_cast<int64_t>(r) * ldq, bx * kBlock8, cols, l16, v[i], s.inv);
+    }
+    if (threadIdx.x == 0) scales[bx * lds + by] = s.s;
+    if (!kAhead) break;
   }
-  if (threadIdx.x == 0) scales[blockIdx.x * lds + blockIdx.y] = s.s;
 }
 
 static bool rows_aligned(const void* p, int64_t ld, size_t size, size_t to) {
@@ -110,16 +132,19 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
   const bool vec = rows_aligned(x, ldx, sizeof(T), 16) && rows_aligned(q, ldq, 1, 8);
   count_launch();
   if (block_rows == 1) {
-    const int groups = (rows + kWarps8 * kRows8 - 1) / (kWarps8 * kRows8);
-    const int chunks = (cols + 2 * kBlock8 - 1) / (2 * kBlock8);
+    const bool narrow = cols <= kBlock8;
+    const int per_block = kWarps8 * kRows8 * (narrow ? 2 : 1);
+    const int groups = (rows + per_block - 1) / per_block, chunks = (cols + 2 * kBlock8 - 1) / (2 * kBlock8);
     const int resident = std::max(1, kBlocksPerSm8 * 148 / chunks);  // blocks per column chunk that run at one time
     const dim3 grid(std::min(groups, resident), chunks);
-    auto k = vec ? quant_rows_kernel<T, true> : quant_rows_kernel<T, false>;
+    auto k = vec ? (narrow ? quant_rows_kernel<T, true, true> : quant_rows_kernel<T, true, false>)
+                 : (narrow ? quant_rows_kernel<T, false, true> : quant_rows_kernel<T, false, false>);
     k<<<grid, kWarps8 * 32, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds);
   } else {
-    const dim3 grid((cols + kBlock8 - 1) / kBlock8, (rows + kBlock8 - 1) / kBlock8);
+    const int blocks_x = (cols + kBlock8 - 1) / kBlock8;
+    const int blocks = blocks_x * ((rows + kBlock8 - 1) / kBlock8);
     auto k = vec ? quant_tiles_kernel<T, true> : quant_tiles_kernel<T, false>;
-    k<<<grid, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds);
+    k<<<sizeof(T) == 2 ? std::min(blocks, 2 * 148) : blocks, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds, blocks_x, blocks);
   }
   return cudaGetLastError();
 }

@@ -163,6 +163,7 @@ __device__ __forceinline__ void load_raw(const T* row, int c0, int cols, int lan
   }
 #pragma unroll
   for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) r.w[j] = make_uint4(0u, 0u, 0u, 0u);
+  if (VEC && c0 + lane * 8 >= cols) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int c = c0 + lane_col<VEC>(lane, j);
@@ -176,9 +177,12 @@ __device__ __forceinline__ void load_cols(const T* row, int c0, int cols, int la
     return;
   }
 #pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+  if (VEC && c0 + lane * 8 >= cols) return;
+#pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int c = c0 + lane_col<VEC>(lane, j);
-    v[j] = c < cols ? to_f32(row[c]) : 0.0f;
+    if (c < cols) v[j] = to_f32(row[c]);
   }
 }
 template <bool VEC, class T>
@@ -187,6 +191,7 @@ __device__ __forceinline__ void store_cols(T* row, int c0, int cols, int lane, c
     store8(row + c0 + lane * 8, v);
     return;
   }
+  if (VEC && c0 + lane * 8 >= cols) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int c = c0 + lane_col<VEC>(lane, j);
@@ -204,6 +209,7 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int 
     *reinterpret_cast<uint2*>(row + c0 + lane * 8) = make_uint2(lo, hi);
     return;
   }
+  if (VEC && c0 + lane * 8 >= cols) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int at = c0 + lane_col<VEC>(lane, j);

@@ -28,7 +28,7 @@ QUANT = dict(x=P, x_type=F32, ldx=256, rows=4, cols=256, block_rows=1, q=P, ldq=
     (dict(cols=0), "cols"), (dict(cols=-5), "cols"), (dict(cols=1 << 24, ldx=1 << 24, ldq=1 << 24), "cols"),
     (dict(block_rows=64), "block_rows"), (dict(block_rows=0), "block_rows"), (dict(q=None), "bad q"),
     (dict(ldq=200), "bad q"), (dict(scales=None), "scales"), (dict(scales=P + 1), "scales"), (dict(lds=3), "scales"),
-    (dict(block_rows=128, rows=1 << 24), "8388480")])
+    (dict(block_rows=128, rows=1 << 30, cols=1 << 20, ldx=1 << 20, ldq=1 << 20, lds=1 << 23), "2^30 blocks")])
 def test_quant8(change, word):
     refused(lbrr.lib().lbrr_op_quant8(*{**QUANT, **change}.values()), "lbrr_op_quant8", word)
 
