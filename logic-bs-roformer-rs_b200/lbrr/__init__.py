@@ -399,17 +399,16 @@ def feed_forward_noalloc(h16, w1, b1, w2, b2, resid, x, stream=None):
 # is a torch.float8_e4m3fn tensor q [rows][cols] and a float32 tensor
 # scales [ceil(cols/128)][ceil(rows/block_rows)].
 # ---------------------------------------------------------------------------
-_torch = None
-_DT = {}     # torch dtype -> LBRR_DT_*
-_F32 = _E4M3 = ()
+_torch = _F32 = _E4M3 = _current_device = None
+_DT = {}  # torch dtype -> LBRR_DT_*
 
 
 def _need_torch():
-    global _torch, _F32, _E4M3
+    global _torch, _F32, _E4M3, _current_device
     if _torch is None:
         import torch
         _DT.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-        _F32, _E4M3 = (torch.float32,), (torch.float8_e4m3fn,)
+        _F32, _E4M3, _current_device = torch.float32, torch.float8_e4m3fn, torch.cuda.current_device
         _torch = torch
     return _torch
 
@@ -428,36 +427,39 @@ def empty8(rows: int, cols: int, block_rows: int = 1, device="cuda"):
     return q, torch.empty(-(-cols // 128), -(-rows // block_rows), dtype=torch.float32, device=device)
 
 
-def _device8(t, name):
-    dev = t.get_device()
+def _matrix(t, name, rows, cols, dtype, dev):
+    """Checks a 2-D tensor and returns the distance between its rows (elements)."""
+    if t.shape == (rows, cols) and t.dtype is dtype and t.get_device() == dev >= 0:
+        ld, step = t.stride()
+        if step == 1 or cols == 1:
+            if rows <= 1:
+                return cols + -cols % 16  # no second row: any distance
+            if ld >= cols:
+                return ld
+            _bad(f"{name} must not have overlapping rows")
+        _bad(f"{name} must have neighbouring columns next to each other")
+    if tuple(t.shape) != (rows, cols):
+        _bad(f"{name} must have shape {(rows, cols)}, has {tuple(t.shape)}")
+    if t.dtype is not dtype:
+        _bad(f"{name} must be {dtype}, is {t.dtype}")
     if dev < 0:
         _bad(f"{name} must be on a CUDA device")
-    return dev
+    _bad(f"{name} must be on the CUDA device of the first operand ({dev}), is on {t.device}")
 
 
-def _matrix(t, name, rows, cols, dtypes, dev):
-    """Checks a 2-D tensor and returns the distance between its rows (elements)."""
-    if t.shape != (rows, cols):
-        _bad(f"{name} must have shape {(rows, cols)}, has {tuple(t.shape)}")
-    if t.dtype not in dtypes:
-        _bad(f"{name} must be {' or '.join(sorted(map(str, dtypes)))}, is {t.dtype}")
-    if t.get_device() != dev:
-        _bad(f"{name} must be on the CUDA device of the first operand ({dev}), is on {t.device}")
-    ld, step = t.stride()
-    if step != 1 and cols > 1:
-        _bad(f"{name} must have neighbouring columns next to each other")
-    if rows <= 1:
-        return cols + -cols % 16  # no second row: any distance
-    if ld < cols:
-        _bad(f"{name} must not have overlapping rows")
-    return ld
+def _kind(t, name):
+    """LBRR_DT_* of a float32, float16 or bfloat16 tensor."""
+    k = _DT.get(t.dtype)
+    if k is None:
+        _bad(f"{name} must be float32, float16 or bfloat16, is {t.dtype}")
+    return k
 
 
 def _vector(t, name, n, dev):
     """Address of a contiguous float32 vector on the device, None for None."""
     if t is None:
         return None
-    if t.shape != (n,) or t.dtype not in _F32 or (n > 1 and t.stride(0) != 1):
+    if t.shape != (n,) or t.dtype is not _F32 or (n > 1 and t.stride(0) != 1):
         _bad(f"{name} must be a contiguous float32 tensor of {n} values")
     if t.get_device() != dev:
         _bad(f"{name} must be on the CUDA device of the first operand ({dev}), is on {t.device}")
@@ -477,30 +479,35 @@ def _same_rows(name, t, ld, other_name, other, other_ld):
 
 def _call8(dev, stream, fn, *args):
     """Calls an entry point with the operands' device current."""
-    torch = _torch
-    if stream is not None and getattr(stream, "device_index", dev) != dev:
-        _bad(f"the stream belongs to device {stream.device_index}, the operands to device {dev}")
-    if torch.cuda.current_device() == dev:
-        rc = fn(*args, _stream(stream))
+    if stream is None:
+        h = None
     else:
-        with torch.cuda.device(dev):
-            rc = fn(*args, _stream(stream))
-    if rc != OK:
+        if getattr(stream, "device_index", dev) != dev:
+            _bad(f"the stream belongs to device {stream.device_index}, the operands to device {dev}")
+        h = _stream(stream)
+    if _current_device() == dev:
+        rc = fn(*args, h)
+    else:
+        with _torch.cuda.device(dev):
+            rc = fn(*args, h)
+    if rc:
         check(rc)
 
 
 def quant8(x, q, scales, block_rows: int = 1, stream=None):
     """x [rows][cols] (float32, float16 or bfloat16) -> q, scales by blocks of
     block_rows (1: activations, 128: weights) x 128."""
-    _need_torch()
+    if _torch is None:
+        _need_torch()
     if x.dim() != 2 or block_rows not in (1, 128):
         _bad("quant8: needs a matrix x and block_rows 1 or 128")
     rows, cols = x.shape
-    dev = _device8(x, "x")
-    ldx = _matrix(x, "x", rows, cols, _DT, dev)
+    dev, dt = x.get_device(), x.dtype
+    kind = _kind(x, "x")
+    ldx = _matrix(x, "x", rows, cols, dt, dev)
     ldq = _matrix(q, "q", rows, cols, _E4M3, dev)
-    lds = _matrix(scales, "scales", -(-cols // 128), -(-rows // block_rows), _F32, dev)
-    _call8(dev, stream, lib().lbrr_op_quant8, x.data_ptr(), _DT[x.dtype], ldx, rows, cols, block_rows, q.data_ptr(),
+    lds = _matrix(scales, "scales", (cols + 127) >> 7, rows if block_rows == 1 else (rows + 127) >> 7, _F32, dev)
+    _call8(dev, stream, (_lib or lib()).lbrr_op_quant8, x.data_ptr(), kind, ldx, rows, cols, block_rows, q.data_ptr(),
            ldq, scales.data_ptr(), lds)
 
 
@@ -508,44 +515,49 @@ def add_norm_quant8(x, resid, gamma, y, q, scales, eps: float = 0.0, stream=None
     """y = x + resid; RMSNorm(y) * gamma -> q, scales by 1 x 128.  resid (x's dtype
     or float32) None: the norm of x, y None.  y (resid's dtype) may be resid or x;
     None: the sum is not stored."""
-    _need_torch()
+    if _torch is None:
+        _need_torch()
     if x.dim() != 2:
         _bad("add_norm_quant8: x must be a matrix")
     rows, cols = x.shape
-    dev = _device8(x, "x")
-    ldx = _matrix(x, "x", rows, cols, _DT, dev)
-    xt = rt = x.dtype
+    dev, xt = x.get_device(), x.dtype
+    kind = rkind = _kind(x, "x")
+    ldx = _matrix(x, "x", rows, cols, xt, dev)
     presid, ldr, py, ldy = None, 0, None, 0
     if resid is not None:
         rt = resid.dtype
-        ldr = _matrix(resid, "resid", rows, cols, (xt,) + _F32, dev)
+        if rt is not xt and rt is not _F32:
+            _bad(f"resid must be {xt} or torch.float32, is {rt}")
+        rkind = _DT[rt]
+        ldr = _matrix(resid, "resid", rows, cols, rt, dev)
         presid = resid.data_ptr()
     if y is not None:
         if resid is None:
             _bad("y (the sum) needs resid")
-        ldy = _matrix(y, "y", rows, cols, (rt,), dev)
+        ldy = _matrix(y, "y", rows, cols, rt, dev)
         py = y.data_ptr()
         _same_rows("y", y, ldy, "x", x, ldx)
         _same_rows("y", y, ldy, "resid", resid, ldr)
     pgamma = _vector(gamma, "gamma", cols, dev)
     ldq = _matrix(q, "q", rows, cols, _E4M3, dev)
-    lds = _matrix(scales, "scales", -(-cols // 128), rows, _F32, dev)
-    _call8(dev, stream, lib().lbrr_op_add_norm_quant8, x.data_ptr(), _DT[xt], ldx, presid, _DT[rt], ldr, pgamma, eps,
-           py, ldy, q.data_ptr(), ldq, scales.data_ptr(), lds, rows, cols)
+    lds = _matrix(scales, "scales", (cols + 127) >> 7, rows, _F32, dev)
+    _call8(dev, stream, (_lib or lib()).lbrr_op_add_norm_quant8, x.data_ptr(), kind, ldx, presid, rkind, ldr, pgamma,
+           eps, py, ldy, q.data_ptr(), ldq, scales.data_ptr(), lds, rows, cols)
 
 
 def _product8(a, a_scales, w, w_scales, bias):
-    _need_torch()
+    if _torch is None:
+        _need_torch()
     if a.dim() != 2 or w.dim() != 2:
         _bad("a and w must be matrices")
     m, k = a.shape
     n = w.shape[0]
-    dev = _device8(a, "a")
-    kb = -(-k // 128)
+    dev = a.get_device()
+    kb = (k + 127) >> 7
     lda = _matrix(a, "a", m, k, _E4M3, dev)
     ldw = _matrix(w, "w", n, k, _E4M3, dev)
     ldas = _matrix(a_scales, "a_scales", kb, m, _F32, dev)
-    ldws = _matrix(w_scales, "w_scales", kb, -(-n // 128), _F32, dev)
+    ldws = _matrix(w_scales, "w_scales", kb, (n + 127) >> 7, _F32, dev)
     return dev, m, n, k, (a.data_ptr(), lda, a_scales.data_ptr(), ldas, w.data_ptr(), ldw, w_scales.data_ptr(), ldws,
                           _vector(bias, "bias", n, dev))
 
@@ -555,15 +567,16 @@ def gemm8(a, a_scales, w, w_scales, out, bias=None, resid=None, stream=None):
     128 x 128.  out: float32, float16 or bfloat16; resid has its dtype and may be
     out itself; bias is float32 [n]."""
     dev, m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
-    ldo = _matrix(out, "out", m, n, _DT, dev)
-    dt = out.dtype
+    kind, dt = _kind(out, "out"), out.dtype
+    ldo = _matrix(out, "out", m, n, dt, dev)
     presid, ldr = None, 0
     if resid is not None:
-        ldr = _matrix(resid, "resid", m, n, (dt,), dev)
+        ldr = _matrix(resid, "resid", m, n, dt, dev)
         presid = resid.data_ptr()
         if m > 0:
             _same_rows("out", out, ldo, "resid", resid, ldr)
-    _call8(dev, stream, lib().lbrr_op_gemm8, *operands, presid, ldr, out.data_ptr(), _DT[dt], ldo, m, n, k)
+    _call8(dev, stream, (_lib or lib()).lbrr_op_gemm8, *operands, presid, ldr, out.data_ptr(),
+           kind, ldo, m, n, k)
 
 
 def gemm8_gelu_quant8(a, a_scales, w, w_scales, bias, q, scales, stream=None):
@@ -571,8 +584,9 @@ def gemm8_gelu_quant8(a, a_scales, w, w_scales, bias, q, scales, stream=None):
     bias float32 [n] or None."""
     dev, m, n, k, operands = _product8(a, a_scales, w, w_scales, bias)
     ldq = _matrix(q, "q", m, n, _E4M3, dev)
-    lds = _matrix(scales, "scales", -(-n // 128), m, _F32, dev)
-    _call8(dev, stream, lib().lbrr_op_gemm8_gelu_quant8, *operands, q.data_ptr(), ldq, scales.data_ptr(), lds, m, n, k)
+    lds = _matrix(scales, "scales", (n + 127) >> 7, m, _F32, dev)
+    _call8(dev, stream, (_lib or lib()).lbrr_op_gemm8_gelu_quant8, *operands, q.data_ptr(), ldq, scales.data_ptr(),
+           lds, m, n, k)
 
 
 def f32_to_f16_bits(v: float) -> int:
