@@ -33,36 +33,26 @@
 
 namespace lbrr {
 
-constexpr int kM8 = 128, kK8 = 128;
+constexpr int kM8 = 128, kN8 = 256, kK8 = 128;
 constexpr int kStages8 = 4;
+constexpr int kABytes8 = kM8 * kK8, kWBytes8 = kN8 / 2 * kK8;  // a CTA's rows of A, its half of the tile's W rows
+constexpr int kStageBytes8 = kABytes8 + kWBytes8;
 constexpr int kOutWarps8 = 8;
-constexpr int kPart8 = 128;                      // columns of an output warp
-constexpr int kBuf8Words = 1024;                 // 32 rows x 128 bytes; two per output warp
-constexpr int kRing8 = 8, kAhead8 = 4;           // K-blocks of scales (and tiles of bias) held, and fetched ahead
+constexpr int kPart8 = 128, kParts8 = kN8 / kPart8;  // columns of an output warp; output warps per TMEM lane quadrant
+constexpr int kBufBytes8 = 4096;                     // 32 rows x 128 bytes; two per output warp
+constexpr int kBufOff8 = kStages8 * kStageBytes8;
+constexpr int kRing8 = 8, kAhead8 = 4;               // K-blocks of scales (and tiles of bias) held, and fetched ahead
+constexpr int kBlockFloats8 = kM8 + 4;               // a K-block: 128 rows' scales, then W's of the two parts
+constexpr int kRingOff8 = kBufOff8 + kOutWarps8 * 2 * kBufBytes8;
+constexpr int kBiasOff8 = kRingOff8 + kRing8 * kBlockFloats8 * 4;
+constexpr int kBarOff8 = kBiasOff8 + kRing8 * kN8 * 4;
+constexpr int kSmem8 = kBarOff8 + 256;
 constexpr int kThreads8 = kOutWarps8 * 32 + 128;
 constexpr int kLoadWarp8 = kOutWarps8, kMmaWarp8 = kOutWarps8 + 1, kScaleWarp8 = kOutWarps8 + 2;
 constexpr int kRegsOut8 = 216, kRegsOther8 = 72;
 constexpr int kLaunchRegs8 = 168;
+static_assert(kSmem8 <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
 static_assert(kOutWarps8 * 32 * kRegsOut8 + 128 * kRegsOther8 <= kThreads8 * kLaunchRegs8, "register split");
-
-// WIDE: 256 x 256 tiles, all output warps on one tile.  Otherwise 256 x 128
-// tiles, the two sets of four output warps on alternate tiles.
-template <bool WIDE>
-struct Layout8 {
-  static constexpr int kN = WIDE ? 256 : 128;              // tile columns
-  static constexpr int kSets = WIDE ? 1 : 2;               // sets of output warps, each with two accumulators
-  static constexpr int kParts = kN / kPart8;               // output warps per TMEM lane quadrant of a set
-  static constexpr int kABytes = kM8 * kK8, kWBytes = kN / 2 * kK8;  // a CTA's rows of A, its half of the W rows
-  static constexpr int kStageBytes = kABytes + kWBytes;
-  static constexpr int kBufOff = kStages8 * kStageBytes;
-  static constexpr int kBlockFloats = kM8 + 4;             // a K-block: 128 rows' scales, then W's of the parts
-  static constexpr int kRingFloats = kRing8 * (kBlockFloats + kN);  // a set's: scales, then bias
-  static constexpr int kRingOff = kBufOff + kOutWarps8 * 2 * kBuf8Words * 4;
-  static constexpr int kBarOff = kRingOff + kSets * kRingFloats * 4;
-  static constexpr int kSmem = kBarOff + 256;
-  static_assert(kSmem <= 232448, "exceeds the 227 KB per-CTA shared memory limit");
-  static_assert(kSets * 2 * kN == 512, "all of TMEM");
-};
 
 enum class Out8 { F32, F16, BF16, Q8 };
 template <Out8 O>
@@ -96,13 +86,12 @@ struct Params8 {
 // Tiles in groups of kGroup8 row tiles, rows fastest: the pairs running at one
 // time share both their A rows and their W rows in L2.
 constexpr int kGroup8 = 8;
-template <bool WIDE>
 __device__ __forceinline__ void tile8(const Params8& p, int idx, int& m0, int& n0) {
   const int gi = p.per.div(idx), rem = idx - gi * (kGroup8 * p.nt);
   const int rows = p.mt - gi * kGroup8;
   const int n = rows >= kGroup8 ? rem / kGroup8 : rem / rows;
   m0 = (gi * kGroup8 + rem - n * min(rows, kGroup8)) * (2 * kM8);
-  n0 = n * Layout8<WIDE>::kN;
+  n0 = n * kN8;
 }
 
 // Byte o of row r in a buffer of 32 rows of 128 bytes with the TMA 128-byte swizzle.
@@ -137,10 +126,7 @@ __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t 
 }
 
 // Columns of the pair's tile that the MMA computes: whole 32s, 16 per CTA's half of W.
-template <bool WIDE>
-__device__ __forceinline__ int tile_cols8(const Params8& p, int n0) {
-  return min(Layout8<WIDE>::kN, (p.g.n - n0 + 31) & ~31);
-}
+__device__ __forceinline__ int tile_cols8(const Params8& p, int n0) { return min(kN8, (p.g.n - n0 + 31) & ~31); }
 
 // 32 columns of a block's sums, times the block's factor, added to the totals.
 template <int B>
@@ -152,20 +138,26 @@ __device__ __forceinline__ void add_scaled(float2 (&acc)[kPart8 / 2], const uint
         __ffma2_rn(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f, acc[16 * B + i]);
 }
 
-template <Out8 O, bool WIDE>
+// Keeps the compiler from starting on these values before, or leaving them for after, this point.
+template <int N>
+__device__ __forceinline__ void hold(float2* x) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+    asm volatile("" : "+f"(x[i].x), "+f"(x[i].y), "+f"(x[i + 1].x), "+f"(x[i + 1].y), "+f"(x[i + 2].x), "+f"(x[i + 2].y), "+f"(x[i + 3].x), "+f"(x[i + 3].y));
+}
+template <Out8 O>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ Params8 p, int* status) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  using L = Layout8<WIDE>;
   using T = typename OutType<O>::T;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_rank();
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBarOff);  // CTA 0's: both CTAs' loads
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff8);  // CTA 0's: both CTAs' loads
   uint64_t* empty = full + kStages8;
-  uint64_t* acc_full = empty + kStages8;            // [sets][2], the block's sums and its scales
-  uint64_t* acc_empty = acc_full + 2 * L::kSets;    // [sets][2], CTA 0's: both CTAs' output warps
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2 * L::kSets);
+  uint64_t* acc_full = empty + kStages8;  // [2], the block's sums and its scales
+  uint64_t* acc_empty = acc_full + 2;     // [2], CTA 0's: both CTAs' output warps
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   if ((smem_u32(smem) & 1023u) != 0) {  // the same in both CTAs: nothing allocated yet
@@ -177,9 +169,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
-    for (int s = 0; s < 2 * L::kSets; ++s) {
+    for (int s = 0; s < 2; ++s) {
       mbar_init(&acc_full[s], 2);
-      mbar_init(&acc_empty[s], 2 * kOutWarps8 / L::kSets);
+      mbar_init(&acc_empty[s], 2 * kOutWarps8);
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -203,16 +195,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       bool ok = true;
       for (int tile = first; ok && tile < n_tiles; tile += step) {
         int m0, n0;
-        tile8<WIDE>(p, tile, m0, n0);
-        const int a_row = m0 + rank * kM8, w_row = n0 + rank * (tile_cols8<WIDE>(p, n0) / 2);
+        tile8(p, tile, m0, n0);
+        const int a_row = m0 + rank * kM8, w_row = n0 + rank * (tile_cols8(p, n0) / 2);
         for (int kb = 0; kb < p.kb; ++kb, ++c) {
           const int s = c % kStages8;
           if (!(ok = mbar_wait(&empty[s], ((c / kStages8) & 1) ^ 1u, abort_flag, status))) break;
-          uint8_t* sa = smem + s * L::kStageBytes;
+          uint8_t* sa = smem + s * kStageBytes8;
           const uint32_t bar = map_to_rank(&full[s], 0);
-          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * L::kStageBytes);
+          if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * kStageBytes8);
           tma_load_2d_pair(sa, &tmA, bar, kb * kK8, a_row);
-          tma_load_2d_pair(sa + L::kABytes, &tmW, bar, kb * kK8, w_row);
+          tma_load_2d_pair(sa + kABytes8, &tmW, bar, kb * kK8, w_row);
         }
       }
       if (!ok && rank == 0) {  // the pair's copies in flight land before its shared memory goes
@@ -225,115 +217,103 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
   } else if (warp == kMmaWarp8) {
     if (rank == 0) {  // the whole warp, so that descriptors and addresses stay uniform; one lane issues
       const uint32_t leader = elect_one();
-      uint32_t c = 0, blocks[2] = {0, 0};  // K-blocks, and those of each set of output warps
-      bool ok = true, loaded = false;      // loaded: block c's operands were seen to have landed
-      int set = 0;
-      for (int tile = first; ok && tile < n_tiles; tile += step, set ^= L::kSets - 1) {
+      uint32_t c = 0;
+      bool ok = true, loaded = false;  // loaded: block c's operands were seen to have landed
+      for (int tile = first; ok && tile < n_tiles; tile += step) {
         int m0, n0;
-        tile8<WIDE>(p, tile, m0, n0);
-        const uint32_t idesc = idesc_e4m3_f32(2 * kM8, tile_cols8<WIDE>(p, n0));
-        uint32_t cs = set ? blocks[1] : blocks[0];
-        for (int kb = 0; kb < p.kb; ++kb, ++c, ++cs) {
-          const int s = c % kStages8, slot = set * 2 + (cs & 1);
+        tile8(p, tile, m0, n0);
+        const uint32_t idesc = idesc_e4m3_f32(2 * kM8, tile_cols8(p, n0));
+        for (int kb = 0; kb < p.kb; ++kb, ++c) {
+          const int s = c % kStages8, slot = c & 1;
           // the accumulator, waited for last, is what the MMAs usually wait for
           if (!__all_sync(0xffffffffu, loaded) &&
               !(ok = mbar_wait(&full[s], (c / kStages8) & 1, abort_flag, status)))
             break;
-          if (!(ok = mbar_wait(&acc_empty[slot], ((cs >> 1) & 1) ^ 1u, abort_flag, status))) break;
+          if (!(ok = mbar_wait(&acc_empty[slot], ((c >> 1) & 1) ^ 1u, abort_flag, status))) break;
           __syncwarp();
           tc_fence_after();
-          const uint64_t da = sdesc_sw128(smem_u32(smem) + s * L::kStageBytes, 1024, 16);
+          const uint64_t da = sdesc_sw128(smem_u32(smem) + s * kStageBytes8, 1024, 16);
 #pragma unroll
           for (int k = 0; k < kK8 / 32; ++k)  // 32 bytes along a row, in the descriptors' units of 16
-            mma_f8_ss_pair(leader, tmem + slot * L::kN, da + k * 2, da + L::kABytes / 16 + k * 2, idesc,
+            mma_f8_ss_pair(leader, tmem + slot * kN8, da + k * 2, da + kABytes8 / 16 + k * 2, idesc,
                            k != 0 ? 1u : 0u);
           mma_commit_pair(leader, &acc_full[slot]);
           mma_commit_pair(leader, &empty[s]);
           loaded = mbar_test(&full[(c + 1) % kStages8], ((c + 1) / kStages8) & 1);
         }
-        if (set)
-          blocks[1] = cs;
-        else
-          blocks[0] = cs;
       }
     }
-  } else if (warp >= kScaleWarp8) {
-    // One warp per set copies its blocks' scales and, with a tile's first block, the tile's bias.  The copies for
-    // block c + kAhead8 are issued once block c - 2's sums are complete: the accumulator of block c - 2 was then
-    // free, so every output warp is done with block c - 4 and has read the bias of its tile; theirs are the
-    // places that are written.
-    const int set = warp - kScaleWarp8;
-    if (set < L::kSets) {
-      float* ring = reinterpret_cast<float*>(smem + L::kRingOff) + set * L::kRingFloats;
-      float* bias_ring = ring + kRing8 * L::kBlockFloats;
-      uint64_t* sums = acc_full + 2 * set;
-      uint32_t issued = 0, i_bias = 0;
-      int i_tile = first + set * step, i_kb = 0, m0 = 0, n0 = 0;
-      const float *a = nullptr, *w = nullptr;
-      auto issue = [&]() {
-        if (i_tile < n_tiles) {
-          if (i_kb == 0) {
-            tile8<WIDE>(p, i_tile, m0, n0);
-            m0 += rank * kM8;
-            a = p.g.a_scales + m0;
-            w = p.g.w_scales + n0 / kBlock8;
-            const int left = p.g.bias ? p.g.n - n0 : 0;  // without a bias: zeros
-            float* dst = bias_ring + i_bias++ % kRing8 * L::kN;
+  } else if (warp == kScaleWarp8) {
+    // The blocks' scales and, with a tile's first block, the tile's bias.  The copies for block c + kAhead8 are
+    // issued once block c - 2's sums are complete: the accumulator of block c - 2 was then free, so every output
+    // warp is done with block c - 4 and has read the bias of its tile; theirs are the places that are written.
+    float* ring = reinterpret_cast<float*>(smem + kRingOff8);
+    float* bias_ring = reinterpret_cast<float*>(smem + kBiasOff8);
+    uint32_t issued = 0, i_bias = 0;
+    int i_tile = first, i_kb = 0, m0 = 0, n0 = 0;
+    const float *a = nullptr, *w = nullptr;
+    auto issue = [&]() {
+      if (i_tile < n_tiles) {
+        if (i_kb == 0) {
+          tile8(p, i_tile, m0, n0);
+          m0 += rank * kM8;
+          a = p.g.a_scales + m0;
+          w = p.g.w_scales + n0 / kBlock8;
+          const int left = p.g.bias ? p.g.n - n0 : 0;  // without a bias: zeros
+          float* dst = bias_ring + i_bias++ % kRing8 * kN8;
 #pragma unroll
-            for (int j = 0; j < L::kN / 32; ++j) {
-              const int cc = lane + 32 * j;
-              cp_async4(dst + cc, cc < left ? p.g.bias + n0 + cc : p.g.a_scales, cc < left);
-            }
+          for (int j = 0; j < kN8 / 32; ++j) {
+            const int cc = lane + 32 * j;
+            cp_async4(dst + cc, cc < left ? p.g.bias + n0 + cc : p.g.a_scales, cc < left);
           }
-          float* dst = ring + issued % kRing8 * L::kBlockFloats;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = lane + 32 * j;
-            const bool in = m0 + r < p.g.m;
-            cp_async4(dst + r, in ? a + r : p.g.a_scales, in);
-          }
-          if (lane < L::kParts) {
-            const bool in = n0 + lane * kPart8 < p.g.n;
-            cp_async4(dst + kM8 + lane, in ? w + lane : p.g.w_scales, in);
-          }
-          a += p.g.ldas;
-          w += p.g.ldws;
-          if (++i_kb == p.kb) {
-            i_kb = 0;
-            i_tile += step * L::kSets;
-          }
-          ++issued;
         }
-        cp_async_commit();
-      };
-      for (int i = 0; i < kAhead8; ++i) issue();
-      for (uint32_t c = 0; c < issued; ++c) {
-        cp_async_wait<kAhead8 - 1>();
-        __syncwarp();
-        const int slot = c & 1;
-        if (c >= 2 && !mbar_wait(&sums[slot], ((c - 2) >> 1) & 1, abort_flag, status)) break;
-        if (lane == 0) mbar_arrive(&sums[slot]);
-        issue();
+        float* dst = ring + issued % kRing8 * kBlockFloats8;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int r = lane + 32 * j;
+          const bool in = m0 + r < p.g.m;
+          cp_async4(dst + r, in ? a + r : p.g.a_scales, in);
+        }
+        if (lane < kParts8) {
+          const bool in = n0 + lane * kPart8 < p.g.n;
+          cp_async4(dst + kM8 + lane, in ? w + lane : p.g.w_scales, in);
+        }
+        a += p.g.ldas;
+        w += p.g.ldws;
+        if (++i_kb == p.kb) {
+          i_kb = 0;
+          i_tile += step;
+        }
+        ++issued;
       }
-      cp_async_wait<0>();
+      cp_async_commit();
+    };
+    for (int i = 0; i < kAhead8; ++i) issue();
+    for (uint32_t c = 0; c < issued; ++c) {
+      cp_async_wait<kAhead8 - 1>();
+      __syncwarp();
+      const int slot = c & 1;
+      if (c >= 2 && !mbar_wait(&acc_full[slot], ((c - 2) >> 1) & 1, abort_flag, status)) break;
+      if (lane == 0) mbar_arrive(&acc_full[slot]);
+      issue();
     }
-  } else {
+    cp_async_wait<0>();
+  } else if (warp < kOutWarps8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsOut8));
-    const int quad = warp & 3, set = WIDE ? 0 : warp >> 2, part = WIDE ? warp >> 2 : 0;
-    uint64_t* sums = acc_full + 2 * set;
-    const uint32_t acc_free = map_to_rank(acc_empty + 2 * set, 0);
-    const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16) + set * 2 * L::kN + part * kPart8;
-    uint8_t* bufs = smem + L::kBufOff + warp * 2 * kBuf8Words * 4;
-    const float* ring = reinterpret_cast<const float*>(smem + L::kRingOff) + set * L::kRingFloats;
-    const float* bias_ring = ring + kRing8 * L::kBlockFloats + part * kPart8;
+    const int quad = warp & 3, part = warp >> 2;
+    const uint32_t acc_free = map_to_rank(acc_empty, 0);
+    const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16) + part * kPart8;
+    uint8_t* bufs = smem + kBufOff8 + warp * 2 * kBufBytes8;
+    const float* ring = reinterpret_cast<const float*>(smem + kRingOff8);
+    const float* bias_ring = reinterpret_cast<const float*>(smem + kBiasOff8) + part * kPart8;
     constexpr int E = 128 / sizeof(T);    // output columns per buffer
     constexpr int kBlocks = kPart8 / E;   // buffers per tile
-    uint32_t c = 0, i_tile = 0;           // this set's K-blocks and tiles
+    uint32_t c = 0, i_tile = 0;
     const uint32_t leader = elect_one();
     bool ok = true;
-    for (int tile = first + set * step; tile < n_tiles; tile += step * L::kSets, ++i_tile) {
+    for (int tile = first; tile < n_tiles; tile += step, ++i_tile) {
       int m0, n0;
-      tile8<WIDE>(p, tile, m0, n0);
+      tile8(p, tile, m0, n0);
       m0 += rank * kM8 + quad * 32;
       n0 += part * kPart8;
       const int cols = p.g.n - n0;  // columns left from this warp's first
@@ -343,7 +323,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       // the other two once the first two have left.
       auto fetch_resid = [&](int b) {
         if (b * E < cols)
-          load_block(bufs + (b & 1) * kBuf8Words * 4,
+          load_block(bufs + (b & 1) * kBufBytes8,
                      static_cast<const T*>(p.g.resid) + static_cast<int64_t>(m0) * p.g.ldr + n0 + b * E, p.g.ldr, rows,
                      cols - b * E, p.resid_vec, lane);
         cp_async_commit();
@@ -365,29 +345,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       auto begin = [&](bool a, bool b) {  // first loads of block c, whose barrier has completed
         if (a) {
           tc_fence_after();
-          const float* sp = ring + c % kRing8 * L::kBlockFloats;
+          const float* sp = ring + c % kRing8 * kBlockFloats8;
           f = sp[quad * 32 + lane] * sp[kM8 + part];
-          tmem_ld32_converged(tm + (c & 1) * L::kN, va);
+          tmem_ld32_converged(tm + (c & 1) * kN8, va);
         }
-        if (b) tmem_ld32_converged(tm + (c & 1) * L::kN + 32, vb);
+        if (b) tmem_ld32_converged(tm + (c & 1) * kN8 + 32, vb);
       };
       auto wait_sums = [&]() {
-        ok = mbar_wait(&sums[c & 1], (c >> 1) & 1, abort_flag, status);
+        ok = mbar_wait(&acc_full[c & 1], (c >> 1) & 1, abort_flag, status);
         __syncwarp();
         return ok;
       };
       if (!wait_sums()) break;
       if (live) {
-        begin(true, true);
-        const float* bias = bias_ring + i_tile % kRing8 * L::kN;  // the totals start from the bias
+        const float* bias = bias_ring + i_tile % kRing8 * kN8;  // the totals start from the bias
 #pragma unroll
         for (int i = 0; i < kPart8 / 4; ++i) {
           const float4 v = *reinterpret_cast<const float4*>(bias + 4 * i);
           acc[2 * i] = make_float2(v.x, v.y);
           acc[2 * i + 1] = make_float2(v.z, v.w);
         }
+        begin(true, true);
         for (int kb = 0;;) {
-          const uint32_t t = tm + (c & 1) * L::kN, freed = acc_free + (c & 1) * 8;
+          const uint32_t t = tm + (c & 1) * kN8, freed = acc_free + (c & 1) * 8;
           const float f0 = f;
           tmem_ld_wait(va);
           tmem_ld_wait(vb);
@@ -397,7 +377,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
           tmem_ld32_converged(t + 96, vb);
           ++c;
           const bool more = ++kb < p.kb;
-          const bool ready = more && mbar_test(&sums[c & 1], (c >> 1) & 1);
+          const bool ready = more && mbar_test(&acc_full[c & 1], (c >> 1) & 1);
           tmem_ld_wait(va);
           tmem_ld_wait(vb);
           tc_fence_before();  // all read: the accumulator is free before the last multiplications
@@ -428,18 +408,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       float inv = 0.0f;
       if constexpr (O == Out8::Q8) {
         float top = 0.0f;
-        if (cols >= kPart8) {
+        if (cols < kPart8) {
 #pragma unroll
           for (int i = 0; i < kPart8 / 2; ++i) {
-            acc[i] = gelu8(acc[i]);
-            top = max_mag3(top, acc[i].x, acc[i].y);
+            if (2 * i >= cols) acc[i].x = 0.0f;
+            if (2 * i + 1 >= cols) acc[i].y = 0.0f;
           }
-        } else {
+        }
 #pragma unroll
-          for (int i = 0; i < kPart8 / 2; ++i) {
-            acc[i] = gelu8(acc[i]);
-            top = max_mag3(top, 2 * i < cols ? acc[i].x : 0.0f, 2 * i + 1 < cols ? acc[i].y : 0.0f);
+        for (int i = 0; i < kPart8 / 2; i += 8) {
+          hold<8>(acc + i);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            acc[i + j] = gelu8(acc[i + j]);
+            top = max_mag3(top, acc[i + j].x, acc[i + j].y);
           }
+          hold<8>(acc + i);
         }
         const Scale8 s = scale8(__float_as_uint(top));
         inv = s.inv;
@@ -465,7 +449,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         }
 #pragma unroll
         for (int b = b0; b < (b0 + 2 < kBlocks ? b0 + 2 : kBlocks); ++b) {
-          uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
+          uint8_t* buf = bufs + (b & 1) * kBufBytes8;
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
             uint4* at = reinterpret_cast<uint4*>(buf + swz(lane, v * 16));
@@ -503,7 +487,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         for (int b = b0; b < (b0 + 2 < kBlocks ? b0 + 2 : kBlocks); ++b) {
           const int cb = b * E;
           if (cb >= cols) break;
-          const uint8_t* buf = bufs + (b & 1) * kBuf8Words * 4;
+          const uint8_t* buf = bufs + (b & 1) * kBufBytes8;
           if (p.out_tma && (cols - cb >= E || p.out_tail)) {
             if (lane == 0) tma_store_2d(&tmOut, buf, n0 + cb, m0);
           } else {
@@ -530,7 +514,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
 }
 
 // Pairs that run at one time on the current device.
-template <bool WIDE>
 static int resident_pairs(const void* kernel) {
   static std::atomic<int> known[64];
   int dev = 0, n = 0;
@@ -541,7 +524,7 @@ static int resident_pairs(const void* kernel) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sms / 2 * 2);
   cfg.blockDim = dim3(kThreads8);
-  cfg.dynamicSmemBytes = Layout8<WIDE>::kSmem;
+  cfg.dynamicSmemBytes = kSmem8;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
   at.val.clusterDim.x = 2;
@@ -556,40 +539,37 @@ static int resident_pairs(const void* kernel) {
   return n;
 }
 
-template <Out8 O, bool WIDE>
+template <Out8 O>
 static cudaError_t launch8(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const Params8& p,
                            int* status, cudaStream_t st) {
-  using L = Layout8<WIDE>;
   static unsigned long long configured = 0;
   cudaError_t e = once_per_device(configured, [] {
-    cudaError_t r = cudaFuncSetAttribute(gemm8_kernel<O, WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem);
+    cudaError_t r = cudaFuncSetAttribute(gemm8_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
     if (r != cudaSuccess) return r;
     // setmaxnreg.inc waits until the block's launch registers cover the split
     cudaFuncAttributes fa;
-    r = cudaFuncGetAttributes(&fa, gemm8_kernel<O, WIDE>);
+    r = cudaFuncGetAttributes(&fa, gemm8_kernel<O>);
     if (r != cudaSuccess) return r;
     return fa.numRegs >= kLaunchRegs8 ? cudaSuccess : cudaErrorInvalidConfiguration;
   });
   if (e != cudaSuccess) return e;
   const int tiles = p.mt * p.nt;
-  const int pairs = resident_pairs<WIDE>(reinterpret_cast<const void*>(gemm8_kernel<O, WIDE>));
+  const int pairs = resident_pairs(reinterpret_cast<const void*>(gemm8_kernel<O>));
   count_launch();
-  gemm8_kernel<O, WIDE><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, L::kSmem, st>>>(ta, tw, to, p, status);
+  gemm8_kernel<O><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
   return cudaGetLastError();
 }
 
-template <bool WIDE>
 static cudaError_t gemm8_tiled(const Gemm8& g, int* status, cudaStream_t st) {
-  using L = Layout8<WIDE>;
   CUtensorMap ta, tw, to;
   Params8 p;
   p.g = g;
   p.mt = (g.m + 2 * kM8 - 1) / (2 * kM8);
-  p.nt = (g.n + L::kN - 1) / L::kN;
+  p.nt = (g.n + kN8 - 1) / kN8;
   p.per = make_fastdiv(static_cast<uint32_t>(kGroup8 * p.nt), static_cast<uint64_t>(p.mt) * p.nt);
   p.kb = (g.k + kK8 - 1) / kK8;
   cudaError_t e = make_map_2d(&ta, g.a, g.k, g.m, g.lda, kK8, kM8, MapElem::U8);
-  if (e == cudaSuccess) e = make_map_2d(&tw, g.w, g.k, g.n, g.ldw, kK8, L::kN / 2, MapElem::U8);
+  if (e == cudaSuccess) e = make_map_2d(&tw, g.w, g.k, g.n, g.ldw, kK8, kN8 / 2, MapElem::U8);
   if (e != cudaSuccess) return e;
   const int size = !g.out ? 1 : g.out_type == Elem::F32 ? 4 : 2;
   const void* dst = g.out ? g.out : g.q;
@@ -603,11 +583,11 @@ static cudaError_t gemm8_tiled(const Gemm8& g, int* status, cudaStream_t st) {
   to = ta;
   if (p.out_tma) e = make_map_2d(&to, dst, g.n, g.m, ld, 128 / size, 32, me);
   if (e != cudaSuccess) return e;
-  if (!g.out) return launch8<Out8::Q8, WIDE>(ta, tw, to, p, status, st);
+  if (!g.out) return launch8<Out8::Q8>(ta, tw, to, p, status, st);
   switch (g.out_type) {
-    case Elem::F32: return launch8<Out8::F32, WIDE>(ta, tw, to, p, status, st);
-    case Elem::F16: return launch8<Out8::F16, WIDE>(ta, tw, to, p, status, st);
-    case Elem::BF16: return launch8<Out8::BF16, WIDE>(ta, tw, to, p, status, st);
+    case Elem::F32: return launch8<Out8::F32>(ta, tw, to, p, status, st);
+    case Elem::F16: return launch8<Out8::F16>(ta, tw, to, p, status, st);
+    case Elem::BF16: return launch8<Out8::BF16>(ta, tw, to, p, status, st);
   }
   return cudaErrorInvalidValue;
 }
@@ -638,7 +618,7 @@ static cudaError_t gemm8_few(const Gemm8& g, int* status, cudaStream_t st) {
 // against 512 x 4096 x 4096 24.5 (18.9), 1024 x 2048 x 2048 15.4 (12.7), 2294 x 1536 x 256 10.2 (7.1).
 cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
   const int64_t tiles = static_cast<int64_t>((g.m + 63) / 64) * ((g.n + 127) / 128);
-  return g.m <= 64 || tiles <= 148 ? gemm8_few(g, status, st) : gemm8_tiled<true>(g, status, st);
+  return g.m <= 64 || tiles <= 148 ? gemm8_few(g, status, st) : gemm8_tiled(g, status, st);
 }
 
 }  // namespace lbrr

@@ -41,6 +41,7 @@ int check_product(const char* op, const uint8_t* a, int64_t lda, const float* a_
   if (!ok_matrix(a_scales, ldas, m, 4)) return bad(op, "bad a_scales");
   if (!ok_matrix(w_scales, ldws, blocks(n), 4)) return bad(op, "bad w_scales");
   if (reinterpret_cast<uintptr_t>(bias) % 4 != 0) return bad(op, "misaligned bias");
+  if (blocks(m) * blocks(n) > (1ll << 30)) return bad(op, "more than 2^30 tiles of 128 x 128");
   return LBRR_OK;
 }
 

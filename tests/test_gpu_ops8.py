@@ -252,7 +252,9 @@ def product(a64, w64, k):
 SHAPES = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (1, 129, 250), (1, 1000, 4096), (2, 256, 300), (7, 64, 128),
           (16, 1024, 256), (17, 130, 640), (33, 515, 127), (62, 1024, 256), (62, 256, 1024), (64, 128, 2048), (65, 384, 384),
           (100, 300, 700), (127, 256, 256), (128, 128, 129), (129, 257, 513), (200, 77, 1500), (255, 1536, 256),
-          (300, 520, 1000), (558, 1536, 256), (1003, 1000, 777), (2294, 256, 1024), (4097, 130, 130), (2048, 2048, 512)]
+          (300, 520, 1000), (558, 1536, 256), (1003, 1000, 777), (2294, 256, 1024), (4097, 130, 130), (2048, 2048, 512),
+          # more tiles than SMs: the tiled kernel, from one K-block to many, ragged rows, columns and K
+          (9999, 260, 100), (30001, 17, 40), (12000, 33, 900), (5000, 700, 129), (2500, 1100, 2100), (19000, 136, 385)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -306,7 +308,7 @@ def test_gemm8_gelu_quant8(lb, m, n, k, with_bias):
     assert canary_kept(buf, m, n)
 
 
-@pytest.mark.parametrize("m,n,k", [(5, 200, 300), (300, 520, 1000), (4097, 130, 130)])
+@pytest.mark.parametrize("m,n,k", [(5, 200, 300), (300, 520, 1000), (4097, 130, 130), (9000, 200, 300)])
 def test_gemm8_adds_into_its_residual(lb, m, n, k):
     a, sa, a64 = operand(lb, m, k, 1, 1)
     w, sw, w64 = operand(lb, n, k, 128, 2)
@@ -345,9 +347,10 @@ def test_gemm8_bad_blocks_stay_in_their_rows(lb, m, n, k):
     assert not torch.isnan(s[0][keep]).any() and not torch.isnan(q[keep][:, cols].float()).any()
 
 
-def test_gemm8_rows_far_apart(lb):
+@pytest.mark.parametrize("m,ld", [(1100, 2 ** 21), (20000, 2 ** 18)])  # split and tiled kernel
+def test_gemm8_rows_far_apart(lb, m, ld):
     """Operand, residual and output offsets past 2^31."""
-    m, n, k, ld = 1100, 136, 260, 2 ** 21
+    n, k = 136, 260
     a, sa, a64 = operand(lb, m, k, 1, 1)
     w, sw, w64 = operand(lb, n, k, 128, 2)
     ab = torch.full((m, ld), 0x7F, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)[:, 64:64 + k]
@@ -357,8 +360,16 @@ def test_gemm8_rows_far_apart(lb):
     h, tol = product(a64, w64, k)
     lb.gemm8(ab, sa, w, sw, out)
     lb.op_sync()
+    assert (m - 1) * ld > 2 ** 31
     assert ((out.double() - h).abs() <= tol + (h.abs() + tol) * 2.0 ** -11 + 2.0 ** -25).all()
-    assert int((ob != 0).sum()) == int((out != 0).sum())
+    assert int(torch.count_nonzero(ob)) == int(torch.count_nonzero(out))
+    x = rnd((m, n), 3, torch.float16)
+    out.copy_(x)
+    lb.gemm8(ab, sa, w, sw, out, resid=out)
+    lb.op_sync()
+    want = h + x.double()
+    lim = tol + 2 * U * (h.abs() + x.double().abs() + tol) + (want.abs() + tol) * 2.0 ** -11 + 2.0 ** -25
+    assert ((out.double() - want).abs() <= lim).all()
 
 
 def test_gemm8_same_bits_every_time(lb):
@@ -463,6 +474,65 @@ def test_side_stream_and_graph_replays(lb):
     feed_forward8(lb, states[0])
     lb.op_sync()
     assert torch.equal(eager, states[0]["y"]) and not torch.equal(eager, want[0])
+
+
+def test_two_products_at_once_on_two_streams(lb):
+    """Tiled and split products of different streams in flight together: each as alone, no shared workspace."""
+    jobs = []
+    for i, (m, n, k) in enumerate([(2294, 1536, 256), (62, 1536, 256), (9000, 520, 300), (1, 4096, 4096)]):
+        a, sa, _ = operand(lb, m, k, 1, 10 + i)
+        w, sw, _ = operand(lb, n, k, 128, 20 + i)
+        want = torch.empty(m, n, device="cuda")
+        lb.gemm8(a, sa, w, sw, want)
+        jobs.append((a, sa, w, sw, want, torch.zeros_like(want), torch.cuda.Stream()))
+    lb.op_sync()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for a, sa, w, sw, _, out, st in jobs:
+            lb.gemm8(a, sa, w, sw, out, stream=st)
+    torch.cuda.synchronize()
+    for *_, want, out, _ in jobs:
+        assert torch.equal(out, want)
+    lb.op_sync()
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import sys
+sys.path.insert(0, sys.argv[1])
+import torch, lbrr
+q, s = lbrr.empty8(4, 128); w, ws = lbrr.empty8(128, 128, 128); out = torch.zeros(4, 128, device="cuda")
+x = torch.ones(128, 128, device="cuda")
+st = torch.cuda.Stream()
+with torch.cuda.stream(st):
+    lbrr.quant8(x[:4], q, s, stream=st); lbrr.quant8(x, w, ws, 128, stream=st)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=st):
+    try:
+        lbrr.gemm8(q, s, w, ws, out, stream=torch.cuda.current_stream())
+        raise SystemExit("not refused")
+    except lbrr.LbrrError as e:
+        assert e.code == lbrr.ERR_STATE and "graph" in str(e), e
+    out.add_(1.0)
+lbrr.gemm8(q, s, w, ws, out, stream=st)
+lbrr.op_sync(st)
+assert (out - 128.0).abs().max() < 1e-3, out
+g.replay()
+torch.cuda.synchronize()
+assert (out - 129.0).abs().max() < 1e-3, out
+print("ok")
+"""
+
+
+def test_first_product_of_a_process_is_refused_inside_a_capture(tmp_path):
+    import subprocess
+    import sys
+    from pathlib import Path
+    pkg = Path(__file__).resolve().parent.parent / "logic-bs-roformer-rs_b200"
+    script = tmp_path / "first_call.py"
+    script.write_text(FIRST_CALL_IN_A_CAPTURE)
+    r = subprocess.run([sys.executable, str(script), str(pkg)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "ok" in r.stdout, r.stdout + r.stderr
 
 
 # ---- refusals that need device tensors ---------------------------------------------

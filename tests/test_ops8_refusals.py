@@ -58,7 +58,7 @@ OPERANDS = [
     (dict(w=None), "16-byte"), (dict(w=P + 1), "16-byte"), (dict(ldw=264), "16-byte"), (dict(a_scales=None), "a_scales"),
     (dict(ldas=7), "a_scales"), (dict(w_scales=None), "w_scales"), (dict(ldws=1), "w_scales"),
     (dict(w_scales=P + 2), "w_scales"), (dict(bias=P + 2), "bias"), (dict(m=-1), "m, n or k"), (dict(n=0), "m, n or k"),
-    (dict(k=0), "m, n or k"), (dict(m=(1 << 30) + 1), "m, n or k"), (dict(k=1 << 24), "m, n or k")]
+    (dict(k=0), "m, n or k"), (dict(m=(1 << 30) + 1), "m, n or k"), (dict(k=1 << 24), "m, n or k"), (dict(m=1 << 30, n=1 << 15, ldas=1 << 30, ldws=256), "2^30 tiles")]
 
 
 @pytest.mark.parametrize("change,word", OPERANDS + [
