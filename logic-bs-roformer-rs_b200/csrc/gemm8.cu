@@ -20,9 +20,10 @@
 // is one number per thread.  After the last block the same warps write the tile
 // through shared memory and TMA stores while the tensor cores run ahead into
 // the next tile.  Warps: 0..7 totals and output, 8 TMA loads, 9 TMEM
-// allocation and (CTA 0) MMA issue, 10 the blocks' scales and 11 the tile's
-// bias (asynchronous copies into rings in shared memory, so the output warps
-// never wait for a global load).
+// allocation and (CTA 0) MMA issue, 10 the tiles' places and bias and the
+// blocks' scales (asynchronous copies into rings in shared memory, so the output
+// warps never wait for a global load), 11 none (it completes the warpgroup that
+// gives its registers away).
 #include <atomic>
 
 #include "cp_async.cuh"
@@ -41,11 +42,12 @@ constexpr int kOutWarps8 = 8;
 constexpr int kPart8 = 128, kParts8 = kN8 / kPart8;  // columns of an output warp; output warps per TMEM lane quadrant
 constexpr int kBufBytes8 = 4096;                     // 32 rows x 128 bytes; two per output warp
 constexpr int kBufOff8 = kStages8 * kStageBytes8;
-constexpr int kRing8 = 8, kAhead8 = 4;               // K-blocks of scales (and tiles of bias) held, and fetched ahead
+constexpr int kRing8 = 8, kAhead8 = 4;               // K-blocks of scales (and tiles) held, and fetched ahead
 constexpr int kBlockFloats8 = kM8 + 4;               // a K-block: 128 rows' scales, then W's of the two parts
 constexpr int kRingOff8 = kBufOff8 + kOutWarps8 * 2 * kBufBytes8;
-constexpr int kBiasOff8 = kRingOff8 + kRing8 * kBlockFloats8 * 4;
-constexpr int kBarOff8 = kBiasOff8 + kRing8 * kN8 * 4;
+constexpr int kTileOff8 = kRingOff8 + kRing8 * kBlockFloats8 * 4;
+constexpr int kTileFloats8 = kN8 + 4;                // a tile: its bias, its first row and column
+constexpr int kBarOff8 = kTileOff8 + kRing8 * kTileFloats8 * 4;
 constexpr int kSmem8 = kBarOff8 + 256;
 constexpr int kThreads8 = kOutWarps8 * 32 + 128;
 constexpr int kLoadWarp8 = kOutWarps8, kMmaWarp8 = kOutWarps8 + 1, kScaleWarp8 = kOutWarps8 + 2;
@@ -80,6 +82,7 @@ struct Params8 {
   bool out_tma;       // the output's rows allow TMA stores
   bool out_tail;      // ... of a last, partial block too: a TMA store ends on a 16-byte boundary, not on the
                       // matrix's last column (measured: it wrote the rest of the 16 bytes)
+  bool out_pairs;     // ... two blocks at a time (tmOut is [blocks][rows][128 bytes])
   bool resid_vec;     // the residual's rows allow 16-byte loads
 };
 
@@ -244,12 +247,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       }
     }
   } else if (warp == kScaleWarp8) {
-    // The blocks' scales and, with a tile's first block, the tile's bias.  The copies for block c + kAhead8 are
-    // issued once block c - 2's sums are complete: the accumulator of block c - 2 was then free, so every output
-    // warp is done with block c - 4 and has read the bias of its tile; theirs are the places that are written.
+    // The blocks' scales and, with a tile's first block, the tile's place and bias.  The copies for block
+    // c + kAhead8 are issued once block c - 2's sums are complete: the accumulator of block c - 2 was then free, so
+    // every output warp is done with block c - 4 and has read what there is of its tile; theirs are the places that
+    // are written.
     float* ring = reinterpret_cast<float*>(smem + kRingOff8);
-    float* bias_ring = reinterpret_cast<float*>(smem + kBiasOff8);
-    uint32_t issued = 0, i_bias = 0;
+    float* tiles = reinterpret_cast<float*>(smem + kTileOff8);
+    uint32_t issued = 0, i_tiles = 0;
     int i_tile = first, i_kb = 0, m0 = 0, n0 = 0;
     const float *a = nullptr, *w = nullptr;
     auto issue = [&]() {
@@ -260,7 +264,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
           a = p.g.a_scales + m0;
           w = p.g.w_scales + n0 / kBlock8;
           const int left = p.g.bias ? p.g.n - n0 : 0;  // without a bias: zeros
-          float* dst = bias_ring + i_bias++ % kRing8 * kN8;
+          float* dst = tiles + i_tiles++ % kRing8 * kTileFloats8;
+          if (lane == 0) *reinterpret_cast<int2*>(dst + kN8) = make_int2(m0, n0);
 #pragma unroll
           for (int j = 0; j < kN8 / 32; ++j) {
             const int cc = lane + 32 * j;
@@ -305,17 +310,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16) + part * kPart8;
     uint8_t* bufs = smem + kBufOff8 + warp * 2 * kBufBytes8;
     const float* ring = reinterpret_cast<const float*>(smem + kRingOff8);
-    const float* bias_ring = reinterpret_cast<const float*>(smem + kBiasOff8) + part * kPart8;
+    const float* tiles = reinterpret_cast<const float*>(smem + kTileOff8);
     constexpr int E = 128 / sizeof(T);    // output columns per buffer
     constexpr int kBlocks = kPart8 / E;   // buffers per tile
     uint32_t c = 0, i_tile = 0;
     const uint32_t leader = elect_one();
     bool ok = true;
+    auto wait_sums = [&]() {
+      ok = mbar_wait(&acc_full[c & 1], (c >> 1) & 1, abort_flag, status);
+      __syncwarp();
+      return ok;
+    };
     for (int tile = first; tile < n_tiles; tile += step, ++i_tile) {
-      int m0, n0;
-      tile8(p, tile, m0, n0);
-      m0 += rank * kM8 + quad * 32;
-      n0 += part * kPart8;
+      if (!wait_sums()) break;
+      const float* bias = tiles + i_tile % kRing8 * kTileFloats8;
+      const int2 at = *reinterpret_cast<const int2*>(bias + kN8);
+      bias += part * kPart8;
+      const int m0 = at.x + quad * 32, n0 = at.y + part * kPart8;
       const int cols = p.g.n - n0;  // columns left from this warp's first
       const int rows = p.g.m - m0;  // rows left from this warp's first
       const bool live = cols > 0 && rows > 0;
@@ -351,15 +362,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         }
         if (b) tmem_ld32_converged(tm + (c & 1) * kN8 + 32, vb);
       };
-      auto wait_sums = [&]() {
-        ok = mbar_wait(&acc_full[c & 1], (c >> 1) & 1, abort_flag, status);
-        __syncwarp();
-        return ok;
-      };
-      if (!wait_sums()) break;
       if (live) {
-        const float* bias = bias_ring + i_tile % kRing8 * kN8;  // the totals start from the bias
-#pragma unroll
+#pragma unroll  // the totals start from the bias
         for (int i = 0; i < kPart8 / 4; ++i) {
           const float4 v = *reinterpret_cast<const float4*>(bias + 4 * i);
           acc[2 * i] = make_float2(v.x, v.y);
@@ -483,10 +487,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
         }
         fence_proxy_async_smem();
         __syncwarp();
+        if (p.out_pairs) {
+          if (lane == 0) tma_store_3d(&tmOut, bufs, 0, m0, (n0 + b0 * E) / E);
+        }
 #pragma unroll
         for (int b = b0; b < (b0 + 2 < kBlocks ? b0 + 2 : kBlocks); ++b) {
           const int cb = b * E;
-          if (cb >= cols) break;
+          if (p.out_pairs || cb >= cols) break;
           const uint8_t* buf = bufs + (b & 1) * kBufBytes8;
           if (p.out_tma && (cols - cb >= E || p.out_tail)) {
             if (lane == 0) tma_store_2d(&tmOut, buf, n0 + cb, m0);
@@ -581,7 +588,12 @@ static cudaError_t gemm8_tiled(const Gemm8& g, int* status, cudaStream_t st) {
                      : size == 4 ? MapElem::F32
                                  : g.out_type == Elem::F16 ? MapElem::F16 : MapElem::BF16;
   to = ta;
-  if (p.out_tma) e = make_map_2d(&to, dst, g.n, g.m, ld, 128 / size, 32, me);
+  const int per_block = 128 / size;
+  p.out_pairs = p.out_tma && size > 1 && g.n % per_block == 0;
+  if (p.out_pairs)
+    e = make_map_3d(&to, dst, per_block, g.m, g.n / per_block, ld, 128, per_block, 32, 2, me);
+  else if (p.out_tma)
+    e = make_map_2d(&to, dst, g.n, g.m, ld, per_block, 32, me);
   if (e != cudaSuccess) return e;
   if (!g.out) return launch8<Out8::Q8>(ta, tw, to, p, status, st);
   switch (g.out_type) {
