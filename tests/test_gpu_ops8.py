@@ -254,7 +254,7 @@ SHAPES = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (1, 129, 250), (1, 1000, 4096),
           (100, 300, 700), (127, 256, 256), (128, 128, 129), (129, 257, 513), (200, 77, 1500), (255, 1536, 256),
           (300, 520, 1000), (558, 1536, 256), (1003, 1000, 777), (2294, 256, 1024), (4097, 130, 130), (2048, 2048, 512),
           # more tiles than SMs: the tiled kernel, from one K-block to many, ragged rows, columns and K
-          (9999, 260, 100), (30001, 17, 40), (12000, 33, 900), (5000, 700, 129), (2500, 1100, 2100), (19000, 136, 385)]
+          (9999, 260, 100), (30001, 17, 40), (12000, 33, 900), (9000, 192, 256), (5000, 700, 129), (2500, 1100, 2100), (19000, 136, 385)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
