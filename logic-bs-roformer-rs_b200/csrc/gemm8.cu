@@ -47,7 +47,8 @@ constexpr int kBlockFloats8 = kM8 + 4;               // a K-block: 128 rows' sca
 constexpr int kRingOff8 = kBufOff8 + kOutWarps8 * 2 * kBufBytes8;
 constexpr int kTileOff8 = kRingOff8 + kRing8 * kBlockFloats8 * 4;
 constexpr int kTileFloats8 = kN8 + 4;                // a tile: its bias, its first row and column
-constexpr int kBarOff8 = kTileOff8 + kRing8 * kTileFloats8 * 4;
+constexpr int kTailOff8 = kTileOff8 + kRing8 * kTileFloats8 * 4;  // 33rd words of the residual's rows, per buffer
+constexpr int kBarOff8 = kTailOff8 + kOutWarps8 * 2 * 32 * 4;
 constexpr int kSmem8 = kBarOff8 + 256;
 constexpr int kThreads8 = kOutWarps8 * 32 + 128;
 constexpr int kLoadWarp8 = kOutWarps8, kMmaWarp8 = kOutWarps8 + 1, kScaleWarp8 = kOutWarps8 + 2;
@@ -83,7 +84,7 @@ struct Params8 {
   bool out_tail;      // ... of a last, partial block too: a TMA store ends on a 16-byte boundary, not on the
                       // matrix's last column (measured: it wrote the rest of the 16 bytes)
   bool out_pairs;     // ... two blocks at a time (tmOut is [blocks][rows][128 bytes])
-  bool resid_vec;     // the residual's rows allow 16-byte loads
+  bool resid_vec;     // the residual's rows allow 16-byte copies
 };
 
 // Tiles in groups of kGroup8 row tiles, rows fastest: the pairs running at one
@@ -102,11 +103,15 @@ __device__ __forceinline__ uint32_t swz(int r, int o) {
   return static_cast<uint32_t>(r * 128 + ((((o >> 4) ^ (r & 7)) << 4) | (o & 15)));
 }
 
-// One 32-row block of 128 bytes per row between global memory and a buffer,
-// coalesced; rows and columns outside the matrix are left alone.
+// One 32-row block of up to 128 bytes per row from global memory to a buffer,
+// asynchronously.  Rows on 16-byte boundaries and whole: 16 bytes a copy.
+// Otherwise 4-byte words: rows of halves that start between words come with the
+// half before them (word j holds halves 2j - 1 and 2j) and their 33rd word goes to
+// `tail`; the reader shifts them.  A word is copied if it holds a value of the
+// block, so no other word is touched.
 template <class T>
-__device__ __forceinline__ void load_block(uint8_t* buf, const T* src, int64_t ld, int rows, int cols, bool vec,
-                                           int lane) {
+__device__ __forceinline__ void load_block(uint8_t* buf, uint32_t* tail, const T* src, int64_t ld, int rows, int cols,
+                                           bool vec, int lane) {
   constexpr int E = 128 / sizeof(T);
   if (vec && cols >= E) {
 #pragma unroll
@@ -116,16 +121,39 @@ __device__ __forceinline__ void load_block(uint8_t* buf, const T* src, int64_t l
     }
     return;
   }
-  for (int r = 0; r < min(rows, 32); ++r)
-    for (int c = lane; c < min(cols, E); c += 32)
-      *reinterpret_cast<T*>(buf + swz(r, c * static_cast<int>(sizeof(T)))) = src[r * ld + c];
+#pragma unroll 4
+  for (int r = 0; r < 32; ++r) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src + r * ld);
+    const int half = (at & 2) != 0;  // never for 32-bit values
+    const int first = lane * (4 / static_cast<int>(sizeof(T))) - half;
+    if (r < rows && first < cols)
+      cp_async4(buf + swz(r, lane * 4), reinterpret_cast<const void*>((at & ~uintptr_t(3)) + lane * 4), true);
+  }
+  if (sizeof(T) == 2 && lane < rows && cols >= E) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(src + lane * ld);
+    if (at & 2) cp_async4(tail + lane, reinterpret_cast<const void*>((at & ~uintptr_t(3)) + 128), true);
+  }
 }
+// ... and back, where a TMA store cannot: in words if the rows start on words, else value by value.
 template <class T>
 __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t ld, int rows, int cols, int lane) {
-  constexpr int E = 128 / sizeof(T);
-  for (int r = 0; r < min(rows, 32); ++r)
-    for (int c = lane; c < min(cols, E); c += 32)
-      dst[r * ld + c] = *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T))));
+  constexpr int E = 128 / sizeof(T), P = 4 / sizeof(T);  // values per row and per word
+  cols = min(cols, E);
+  if (((reinterpret_cast<uintptr_t>(dst) | (static_cast<uintptr_t>(ld) * sizeof(T))) & 3) == 0) {
+    const int words = cols / P;
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
+      if (r < rows && lane < words)
+        *reinterpret_cast<uint32_t*>(dst + r * ld + lane * P) = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
+    for (int c = words * P; c < cols; ++c)
+      if (lane < rows) dst[lane * ld + c] = *reinterpret_cast<const T*>(buf + swz(lane, c * static_cast<int>(sizeof(T))));
+    return;
+  }
+#pragma unroll 8
+  for (int r = 0; r < 32; ++r)
+#pragma unroll
+    for (int c = lane; c < E; c += 32)
+      if (r < rows && c < cols) dst[r * ld + c] = *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T))));
 }
 
 // Columns of the pair's tile that the MMA computes: whole 32s, 16 per CTA's half of W.
@@ -148,7 +176,8 @@ __device__ __forceinline__ void hold(float2* x) {
   for (int i = 0; i < N; i += 4)
     asm volatile("" : "+f"(x[i].x), "+f"(x[i].y), "+f"(x[i + 1].x), "+f"(x[i + 1].y), "+f"(x[i + 2].x), "+f"(x[i + 2].y), "+f"(x[i + 3].x), "+f"(x[i + 3].y));
 }
-template <Out8 O>
+// ODD: a 16-bit residual with rows that may start between 4-byte words.
+template <Out8 O, bool ODD>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     gemm8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmW,
                  const __grid_constant__ CUtensorMap tmOut, const __grid_constant__ Params8 p, int* status) {
@@ -309,6 +338,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
     const uint32_t acc_free = map_to_rank(acc_empty, 0);
     const uint32_t tm = tmem + (static_cast<uint32_t>(quad * 32) << 16) + part * kPart8;
     uint8_t* bufs = smem + kBufOff8 + warp * 2 * kBufBytes8;
+    uint32_t* tails = reinterpret_cast<uint32_t*>(smem + kTailOff8) + warp * 64;
     const float* ring = reinterpret_cast<const float*>(smem + kRingOff8);
     const float* tiles = reinterpret_cast<const float*>(smem + kTileOff8);
     constexpr int E = 128 / sizeof(T);    // output columns per buffer
@@ -334,7 +364,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
       // the other two once the first two have left.
       auto fetch_resid = [&](int b) {
         if (b * E < cols)
-          load_block(bufs + (b & 1) * kBufBytes8,
+          load_block(bufs + (b & 1) * kBufBytes8, tails + (b & 1) * 32,
                      static_cast<const T*>(p.g.resid) + static_cast<int64_t>(m0) * p.g.ldr + n0 + b * E, p.g.ldr, rows,
                      cols - b * E, p.resid_vec, lane);
         cp_async_commit();
@@ -468,6 +498,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
             } else {
               uint4 r = make_uint4(0u, 0u, 0u, 0u);
               if (p.g.resid) r = *at;
+              if constexpr (ODD) {  // the row's halves start in the middle of its first word
+                const T* from = static_cast<const T*>(p.g.resid) + static_cast<int64_t>(m0 + lane) * p.g.ldr + n0;
+                const uint32_t sh = (reinterpret_cast<uintptr_t>(from) & 2) * 8;
+                const uint32_t next = v < 7 ? *reinterpret_cast<const uint32_t*>(buf + swz(lane, v * 16 + 16))
+                                            : tails[(b & 1) * 32 + lane];
+                r = make_uint4(__funnelshift_r(r.x, r.y, sh), __funnelshift_r(r.y, r.z, sh),
+                               __funnelshift_r(r.z, r.w, sh), __funnelshift_r(r.w, next, sh));
+              }
               const uint32_t rw[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -546,24 +584,24 @@ static int resident_pairs(const void* kernel) {
   return n;
 }
 
-template <Out8 O>
+template <Out8 O, bool ODD = false>
 static cudaError_t launch8(const CUtensorMap& ta, const CUtensorMap& tw, const CUtensorMap& to, const Params8& p,
                            int* status, cudaStream_t st) {
   static unsigned long long configured = 0;
   cudaError_t e = once_per_device(configured, [] {
-    cudaError_t r = cudaFuncSetAttribute(gemm8_kernel<O>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
+    cudaError_t r = cudaFuncSetAttribute(gemm8_kernel<O, ODD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem8);
     if (r != cudaSuccess) return r;
     // setmaxnreg.inc waits until the block's launch registers cover the split
     cudaFuncAttributes fa;
-    r = cudaFuncGetAttributes(&fa, gemm8_kernel<O>);
+    r = cudaFuncGetAttributes(&fa, gemm8_kernel<O, ODD>);
     if (r != cudaSuccess) return r;
     return fa.numRegs >= kLaunchRegs8 ? cudaSuccess : cudaErrorInvalidConfiguration;
   });
   if (e != cudaSuccess) return e;
   const int tiles = p.mt * p.nt;
-  const int pairs = resident_pairs(reinterpret_cast<const void*>(gemm8_kernel<O>));
+  const int pairs = resident_pairs(reinterpret_cast<const void*>(gemm8_kernel<O, ODD>));
   count_launch();
-  gemm8_kernel<O><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
+  gemm8_kernel<O, ODD><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
   return cudaGetLastError();
 }
 
@@ -595,11 +633,15 @@ static cudaError_t gemm8_tiled(const Gemm8& g, int* status, cudaStream_t st) {
   else if (p.out_tma)
     e = make_map_2d(&to, dst, g.n, g.m, ld, per_block, 32, me);
   if (e != cudaSuccess) return e;
+  const bool odd = g.resid && size == 2 && (reinterpret_cast<uintptr_t>(g.resid) % 4 != 0 || g.ldr % 2 != 0);
   if (!g.out) return launch8<Out8::Q8>(ta, tw, to, p, status, st);
   switch (g.out_type) {
     case Elem::F32: return launch8<Out8::F32>(ta, tw, to, p, status, st);
-    case Elem::F16: return launch8<Out8::F16>(ta, tw, to, p, status, st);
-    case Elem::BF16: return launch8<Out8::BF16>(ta, tw, to, p, status, st);
+    case Elem::F16:
+      return odd ? launch8<Out8::F16, true>(ta, tw, to, p, status, st) : launch8<Out8::F16>(ta, tw, to, p, status, st);
+    case Elem::BF16:
+      return odd ? launch8<Out8::BF16, true>(ta, tw, to, p, status, st)
+                 : launch8<Out8::BF16>(ta, tw, to, p, status, st);
   }
   return cudaErrorInvalidValue;
 }

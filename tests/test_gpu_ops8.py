@@ -254,7 +254,7 @@ SHAPES = [(1, 1, 1), (1, 16, 16), (1, 128, 128), (1, 129, 250), (1, 1000, 4096),
           (100, 300, 700), (127, 256, 256), (128, 128, 129), (129, 257, 513), (200, 77, 1500), (255, 1536, 256),
           (300, 520, 1000), (558, 1536, 256), (1003, 1000, 777), (2294, 256, 1024), (4097, 130, 130), (2048, 2048, 512),
           # more tiles than SMs: the tiled kernel, from one K-block to many, ragged rows, columns and K
-          (9999, 260, 100), (30001, 17, 40), (12000, 33, 900), (9000, 192, 256), (5000, 700, 129), (2500, 1100, 2100), (19000, 136, 385)]
+          (9999, 260, 100), (30001, 17, 40), (12000, 33, 900), (9000, 192, 256), (9001, 251, 200), (5000, 700, 129), (2500, 1100, 2100), (19000, 136, 385)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -264,12 +264,13 @@ def test_gemm8(lb, m, n, k):
     bias = rnd((1, n), 5)[0]
     h, tol = product(a64, w64, k)
     for i, (kind, with_bias, with_resid, pitch) in enumerate([
-            ("f32", True, True, 0), ("f32", False, False, 3), ("f16", True, False, 8), ("f16", False, True, 0),
-            ("bf16", True, True, 1), ("bf16", False, False, 0)]):
+            ("f32", True, True, 0), ("f32", False, True, 3), ("f16", True, False, 8), ("f16", False, True, 0),
+            ("bf16", True, True, 1), ("bf16", False, False, 0), ("f16", True, True, 2), ("bf16", False, False, 3)]):
         dt = TYPES[kind]
         buf = torch.full((m + 1, n + pitch), 5.0, dtype=dt, device="cuda")
         out = buf[:m, :n]
-        resid = rnd((m, n), 6 + i, dt, pad=pitch) if with_resid else None
+        # residual rows at the output's pitch, starting one value in where there is room
+        resid = rnd((m, n), 6 + i, dt, pad=pitch, shift=min(pitch, i % 2)) if with_resid else None
         lb.gemm8(a, sa, w, sw, out, bias=bias if with_bias else None, resid=resid)
         lb.op_sync()
         want, lim = h, tol
