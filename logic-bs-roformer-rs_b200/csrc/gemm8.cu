@@ -134,26 +134,46 @@ __device__ __forceinline__ void load_block(uint8_t* buf, uint32_t* tail, const T
     if (at & 2) cp_async4(tail + lane, reinterpret_cast<const void*>((at & ~uintptr_t(3)) + 128), true);
   }
 }
-// ... and back, where a TMA store cannot: in words if the rows start on words, else value by value.
+// ... and back, where a TMA store cannot: in words, and single values where a row begins or ends inside one
+// (bytes whose rows do not start on words go one by one).
 template <class T>
 __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t ld, int rows, int cols, int lane) {
   constexpr int E = 128 / sizeof(T), P = 4 / sizeof(T);  // values per row and per word
   cols = min(cols, E);
-  if (((reinterpret_cast<uintptr_t>(dst) | (static_cast<uintptr_t>(ld) * sizeof(T))) & 3) == 0) {
+  auto value = [&](int r, int c) { return *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T)))); };
+  const uintptr_t off = reinterpret_cast<uintptr_t>(dst) | (static_cast<uintptr_t>(ld) * sizeof(T));
+  if ((off & 3) == 0) {
     const int words = cols / P;
 #pragma unroll 8
     for (int r = 0; r < 32; ++r)
       if (r < rows && lane < words)
         *reinterpret_cast<uint32_t*>(dst + r * ld + lane * P) = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
     for (int c = words * P; c < cols; ++c)
-      if (lane < rows) dst[lane * ld + c] = *reinterpret_cast<const T*>(buf + swz(lane, c * static_cast<int>(sizeof(T))));
-    return;
-  }
+      if (lane < rows) dst[lane * ld + c] = value(lane, c);
+  } else if (sizeof(T) == 2) {
+    // rows that start between words: word j of such a row holds columns 2j - 1 and 2j
 #pragma unroll 8
-  for (int r = 0; r < 32; ++r)
+    for (int r = 0; r < 32; ++r) {
+      T* row = dst + r * ld;
+      const int half = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1, c = 2 * lane - half;
+      const uint32_t own = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
+      const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
+      if (r < rows && c >= 0 && c + 1 < cols)
+        *reinterpret_cast<uint32_t*>(row + c) = __funnelshift_l(before, own, half * 16);
+    }
+    if (lane < rows) {
+      T* row = dst + lane * ld;
+      const int half = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1;
+      if (half) row[0] = value(lane, 0);
+      if ((cols + half) & 1) row[cols - 1] = value(lane, cols - 1);
+    }
+  } else {
+#pragma unroll 8
+    for (int r = 0; r < 32; ++r)
 #pragma unroll
-    for (int c = lane; c < E; c += 32)
-      if (r < rows && c < cols) dst[r * ld + c] = *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T))));
+      for (int c = lane; c < E; c += 32)
+        if (r < rows && c < cols) dst[r * ld + c] = value(r, c);
+  }
 }
 
 // Columns of the pair's tile that the MMA computes: whole 32s, 16 per CTA's half of W.
