@@ -2,7 +2,13 @@
 // matrix to e4m3 with scales, and the trunk's RMSNorm with the residual's
 // addition and an 8-bit output.  Both are one pass over their data (every
 // value is read once, held in registers while its block's or row's statistics
-// form, and written once), so HBM bounds them.
+// form, and written once), so HBM bounds them where there are rows enough to
+// fill the GPU.  What made the difference was having the next rows' loads in
+// flight while a block is worked on (71362 x 512 fp16 28 -> 20 us, 5.5 TB/s;
+// norm 4099 x 5000 bf16 46 -> 30 us, 4.8 TB/s) and few instructions per value (a
+// division per block, sixteen compares per eight values and a reduction per
+// block cost 15-25 %).  Norm of 71362 x 256 (fp16 branch, fp32 stream): 33 us,
+// 6.0 TB/s.
 #include <algorithm>
 #include <cmath>
 
