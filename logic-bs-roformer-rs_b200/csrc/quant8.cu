@@ -20,7 +20,8 @@ namespace lbrr {
 // v -> (q, scales), blocks of 1 x 128.  A warp takes kRows8 rows of 256
 // columns (16 lanes per block) at a time and has the next ones' loads in flight
 // meanwhile; eight warps cover 32 rows, so the scales of a block column leave
-// as whole sectors.
+// as whole sectors.  Unaligned rows (Shifted8) leave no registers for the loads
+// ahead: 71362 x 257 fp32 45 us, 53 with them; 37889 x 588 bf16 32 and 33.
 // ---------------------------------------------------------------------------
 constexpr int kRows8 = 4;
 constexpr int kWarps8 = 8;
@@ -30,41 +31,43 @@ constexpr int kBlocksPerSm8 = 4;
 template <class T, bool VEC, bool NARROW>
 __global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
     quant_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
-                      float* __restrict__ scales, int64_t lds) {
+                      float* __restrict__ scales, int64_t lds, bool q_aligned) {
   constexpr int kPerWarp = NARROW ? 2 * kRows8 : kRows8;  // rows
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int half = lane >> 4, at = NARROW ? lane & 15 : lane;  // `at`: this lane's columns
   const int c0 = blockIdx.y * 2 * kBlock8;
+  constexpr bool kAhead = VEC;
   auto row_of = [&](int r0, int i) { return NARROW ? r0 + 2 * i + half : r0 + i; };
-  Raw8<T> next[kRows8];
+  Ahead8<VEC, NARROW ? 16 : 32, T> next[kRows8];
+  auto row_at = [&](int r0, int i) { return x + static_cast<int64_t>(row_of(r0, i)) * ldx; };
   auto fetch = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < kRows8; ++i)
-      if (row_of(r0, i) < rows)
-        load_raw<VEC>(x + static_cast<int64_t>(row_of(r0, i)) * ldx, c0, cols, at, next[i]);
+      if (row_of(r0, i) < rows) next[i].load(row_at(r0, i), c0, cols, at);
   };
   const int step = gridDim.x * kWarps8 * kPerWarp;
   int r0 = (blockIdx.x * kWarps8 + warp) * kPerWarp;
-  fetch(r0);
+  if (kAhead) fetch(r0);
   for (; r0 < rows; r0 += step) {
+    if (!kAhead) fetch(r0);
     float v[kRows8][8];
     uint32_t top[kRows8];
 #pragma unroll
     for (int i = 0; i < kRows8; ++i) {
-      if (row_of(r0, i) < rows) {
-        next[i].get(v[i]);
+      if (!VEC || row_of(r0, i) < rows) {  // rows past the last one: whole warps shift, nothing is stored
+        next[i].get(row_at(r0, i), c0, cols, at, v[i]);
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
       }
       top[i] = top_of(v[i]);
     }
-    fetch(r0 + step);
+    if (kAhead) fetch(r0 + step);
     const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
 #pragma unroll
     for (int i = 0; i < kRows8; ++i)
       if (row_of(r0, i) < rows)
-        store_codes<VEC>(q + static_cast<int64_t>(row_of(r0, i)) * ldq, c0, cols, at, v[i], sc.inv[i]);
+        store_codes<true>(q + static_cast<int64_t>(row_of(r0, i)) * ldq, c0, cols, at, v[i], sc.inv[i], VEC || q_aligned);
     const int own = row_of(r0, sc.own_block), kb = NARROW ? 0 : blockIdx.y * 2 + half;
     if (sc.writer && own < rows && kb * kBlock8 < cols) scales[kb * lds + own] = sc.own;
   }
@@ -72,28 +75,29 @@ __global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
 
 // Blocks of 128 x 128: 32 values per thread.  16-bit inputs: two CTAs per SM
 // walk the blocks with the next one's loads in flight (71362 x 512: 33 -> 22 us);
-// 32-bit inputs leave no registers for that, so each block has its own CTA
-// (8192 x 8192: 51 us, 61 with the loop).  `blocks_x`: blocks side by side.
+// 32-bit inputs and unaligned rows leave no registers for that, so each block has
+// its own CTA (8192 x 8192 fp32: 51 us, 61 with the loop; 9402 x 1227 bf16: 10.6
+// and 16.6).  `blocks_x`: blocks side by side.
 constexpr int kTileThreads8 = 512;
 template <class T, bool VEC>
 __global__ void __launch_bounds__(kTileThreads8, 2)
     quant_tiles_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
-                       float* __restrict__ scales, int64_t lds, int blocks_x, int blocks) {
+                       float* __restrict__ scales, int64_t lds, bool q_aligned, int blocks_x, int blocks) {
   constexpr int kPer = kBlock8 * kBlock8 / kTileThreads8 / 8;  // row groups per thread
   constexpr int kStep = kTileThreads8 / 16;                    // rows per group
   __shared__ uint32_t part[2][kTileThreads8 / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int l16 = lane & 15;  // the 16 lanes of a row
-  Raw8<T> next[kPer];
+  Ahead8<VEC, 16, T> next[kPer];
   auto fetch = [&](int block) {
     const int by = block / blocks_x, c0 = (block - by * blocks_x) * kBlock8;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = by * kBlock8 + (threadIdx.x >> 4) + i * kStep;
-      if (r < rows) load_raw<VEC>(x + static_cast<int64_t>(r) * ldx, c0, cols, l16, next[i]);
+      if (r < rows) next[i].load(x + static_cast<int64_t>(r) * ldx, c0, cols, l16);
     }
   };
-  constexpr bool kAhead = sizeof(T) == 2;
+  constexpr bool kAhead = VEC && sizeof(T) == 2;
   int block = blockIdx.x;
   fetch(block);
   for (int it = 0; block < blocks; block += gridDim.x, it ^= 1) {
@@ -103,9 +107,9 @@ __global__ void __launch_bounds__(kTileThreads8, 2)
     uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (r0 + i * kStep < rows) {
-        next[i].get(v[i]);
-      } else {
+      const int r = r0 + i * kStep;
+      if (!VEC || r < rows) next[i].get(x + static_cast<int64_t>(r) * ldx, bx * kBlock8, cols, l16, v[i]);
+      if (r >= rows) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
       }
@@ -120,7 +124,7 @@ __global__ void __launch_bounds__(kTileThreads8, 2)
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = r0 + i * kStep;
-      if (r < rows) store_codes<VEC>(q + static_cast<int64_t>(r) * ldq, bx * kBlock8, cols, l16, v[i], s.inv);
+      if (r < rows) store_codes<true>(q + static_cast<int64_t>(r) * ldq, bx * kBlock8, cols, l16, v[i], s.inv, VEC || q_aligned);
     }
     if (threadIdx.x == 0) scales[bx * lds + by] = s.s;
     if (!kAhead) break;
@@ -135,7 +139,7 @@ template <class T>
 static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int block_rows, uint8_t* q, int64_t ldq,
                             float* scales, int64_t lds, cudaStream_t st) {
   const T* x = static_cast<const T*>(xv);
-  const bool vec = rows_aligned(x, ldx, sizeof(T), 16) && rows_aligned(q, ldq, 1, 8);
+  const bool q_aligned = rows_aligned(q, ldq, 1, 8), vec = q_aligned && rows_aligned(x, ldx, sizeof(T), 16);
   count_launch();
   if (block_rows == 1) {
     const bool narrow = cols <= kBlock8;
@@ -145,12 +149,13 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
     const dim3 grid(std::min(groups, resident), chunks);
     auto k = vec ? (narrow ? quant_rows_kernel<T, true, true> : quant_rows_kernel<T, true, false>)
                  : (narrow ? quant_rows_kernel<T, false, true> : quant_rows_kernel<T, false, false>);
-    k<<<grid, kWarps8 * 32, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds);
+    k<<<grid, kWarps8 * 32, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds, q_aligned);
   } else {
     const int blocks_x = (cols + kBlock8 - 1) / kBlock8;
     const int blocks = blocks_x * ((rows + kBlock8 - 1) / kBlock8);
     auto k = vec ? quant_tiles_kernel<T, true> : quant_tiles_kernel<T, false>;
-    k<<<sizeof(T) == 2 ? std::min(blocks, 2 * 148) : blocks, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds, blocks_x, blocks);
+    k<<<vec && sizeof(T) == 2 ? std::min(blocks, 2 * 148) : blocks, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds,
+                                                                                   q_aligned, blocks_x, blocks);
   }
   return cudaGetLastError();
 }
@@ -213,13 +218,14 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1)
   const int per_cta = warps == 1 ? blockDim.x >> 5 : 1;
   const int wr = warps == 1 ? 0 : warp;  // this warp's place in its row
   const int step = gridDim.x * per_cta;
+  constexpr bool kUnits = VEC && C == 2;  // 4099 x 5000 fp16 + fp32: 46 -> 42 us; for C = 4, 500 x 24000: 33 -> 38
   Raw8<TX> nx[C];
   Raw8<TR> nr[C];
   auto fetch = [&](int64_t r) {
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      load_raw<VEC>(x + r * ldx, (wr + i * warps) * 256, cols, lane, nx[i]);
-      if (resid) load_raw<VEC>(resid + r * ldr, (wr + i * warps) * 256, cols, lane, nr[i]);
+      load_raw<VEC, kUnits>(x + r * ldx, (wr + i * warps) * 256, cols, lane, nx[i]);
+      if (resid) load_raw<VEC, kUnits>(resid + r * ldr, (wr + i * warps) * 256, cols, lane, nr[i]);
     }
   };
   int64_t row = blockIdx.x * per_cta + (warps == 1 ? warp : 0);
@@ -228,12 +234,16 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1)
   for (;; row += step) {
     float v[C][8];
 #pragma unroll
-    for (int i = 0; i < C; ++i) nx[i].get(v[i]);
+    for (int i = 0; i < C; ++i) {
+      nx[i].get(v[i]);
+      if (kUnits) drop_past((wr + i * warps) * 256, cols, lane, v[i]);
+    }
     if (resid) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         float r[8];
         nr[i].get(r);
+        if (kUnits) drop_past((wr + i * warps) * 256, cols, lane, r);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[i][j] += r[j];
       }
@@ -314,9 +324,11 @@ static cudaError_t add_norm_quant8_t(const AddNorm8& a, cudaStream_t st) {
   const float inv_cols = 1.0f / static_cast<float>(a.cols);
   const float most = static_cast<float>(std::sqrt(static_cast<double>(a.cols)) * 1e12);  // 1 / the norm's floor
   count_launch();
-#define LBRR_LAUNCH(CC, LOOP, MAX)                                                                                \
-  (vec ? add_norm_quant_kernel<TX, TR, CC, true, LOOP, MAX> : add_norm_quant_kernel<TX, TR, CC, false, LOOP, MAX>) \
-      <<<grid, threads, 0, st>>>(x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds,   \
+  constexpr bool kAhead = sizeof(TX) + sizeof(TR) < 8;
+#define LBRR_LAUNCH(CC, LOOP, MAX)                                                                          \
+  (vec ? add_norm_quant_kernel<TX, TR, CC, true, LOOP && kAhead, MAX>                                        \
+       : add_norm_quant_kernel<TX, TR, CC, false, false, MAX>)                                               \
+      <<<grid, threads, 0, st>>>(x, a.ldx, resid, a.ldr, a.gamma, a.eps, y, a.ldy, a.q, a.ldq, a.scales, a.lds, \
                                  a.rows, a.cols, warps, inv_cols, most)
   if (chunks <= 2) {  // a warp per row
     constexpr int warps = 1, threads = 128;
@@ -325,9 +337,14 @@ static cudaError_t add_norm_quant8_t(const AddNorm8& a, cudaStream_t st) {
       LBRR_LAUNCH(1, false, threads);
     else
       LBRR_LAUNCH(2, false, threads);
-  } else if (chunks <= 64) {  // a block per row, the next row's loads in flight; as many blocks as run at one time
+  } else if (chunks <= 64) {  // a block per row
+    // As many blocks as run at one time, the next row's loads in flight (4099 x
+    // 5000 bf16: 46 -> 30 us).  Where that needs more registers than there are, as
+    // many blocks as rows: both inputs fp32 (4099 x 5000: 44 us, 57 with loads
+    // ahead), and unaligned rows, which load value by value (9402 x 1227 bf16: 26
+    // and 37).
     const int warps = (chunks + 1) / 2, threads = warps * 32;
-    const int grid = std::min(a.rows, 148 * (1024 / threads));
+    const int grid = vec && kAhead ? std::min(a.rows, 148 * (1024 / threads)) : a.rows;
     if (threads <= 512)
       LBRR_LAUNCH(2, true, 512);
     else

@@ -15,6 +15,8 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 
@@ -153,8 +155,21 @@ struct Raw8 {
     }
   }
 };
-template <bool VEC, class T>
+// UNITS: an aligned row's last 16-byte unit is loaded whole and `drop_past` zeroes
+// what is past the last column; otherwise it is loaded value by value.  Which of
+// the two costs fewer registers depends on the kernel.
+template <bool VEC, bool UNITS = false, class T>
 __device__ __forceinline__ void load_raw(const T* row, int c0, int cols, int lane, Raw8<T>& r) {
+  if constexpr (VEC && UNITS) {
+    constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+    for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j) {
+      const int c = c0 + lane * 8 + j * kPer;
+      r.w[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (c < cols) r.w[j] = *reinterpret_cast<const uint4*>(row + c);
+    }
+    return;
+  }
   if (VEC && c0 + lane * 8 + 8 <= cols) {
 #pragma unroll
     for (int j = 0; j < static_cast<int>(sizeof(T) / 2); ++j)
@@ -170,6 +185,88 @@ __device__ __forceinline__ void load_raw(const T* row, int c0, int cols, int lan
     if (c < cols) r.t[j] = row[c];
   }
 }
+__device__ __forceinline__ void drop_past(int c0, int cols, int lane, float (&v)[8]) {
+  if (c0 + lane * 8 + 8 <= cols) return;
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (c0 + lane * 8 + j >= cols) v[j] = 0.0f;
+}
+// Eight consecutive columns of a row that does not start on a 16-byte boundary,
+// as VEC's lanes hold them.  LANES lanes load the 16-byte units that their
+// columns lie in, the first lane from the unit that column c0 is in, and shift
+// the values into place with the following lane's: as many loads as for an
+// aligned row, where value by value it would be eight (37889 x 588 bf16: 42 -> 32
+// us).  A unit is loaded if it
+// holds a value of the row, so no page without one is touched.
+template <int LANES, class T>
+struct Shifted8 {
+  static constexpr int kUnits = sizeof(T) / 2;  // 16-byte units per lane
+  uint4 unit[kUnits], extra;                    // extra: the unit after the last lane's
+
+  // `lane`: this lane's place among the LANES.
+  __device__ __forceinline__ void load(const T* row, int c0, int cols, int lane) {
+    const int bytes = min(cols - c0, 2 * kBlock8 + 8) * static_cast<int>(sizeof(T));  // of the row, as far as it matters
+    const uintptr_t at = reinterpret_cast<uintptr_t>(row + c0);
+    const int d = static_cast<int>(at & 15);
+    const uint4* from = reinterpret_cast<const uint4*>(at - d);
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j) {
+      const int u = lane * kUnits + j;
+      unit[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (u * 16 - d < bytes) unit[j] = from[u];
+    }
+    extra = make_uint4(0u, 0u, 0u, 0u);
+    if (lane == LANES - 1 && d != 0 && LANES * kUnits * 16 - d < bytes) extra = from[LANES * kUnits];
+  }
+  // The values, zero past the last column; every lane of the warp calls it.
+  __device__ __forceinline__ void get(const T* row, int c0, int cols, int lane, float (&v)[8]) const {
+    uint32_t w[4 * kUnits + 4];
+#pragma unroll
+    for (int j = 0; j < kUnits; ++j)
+      w[4 * j] = unit[j].x, w[4 * j + 1] = unit[j].y, w[4 * j + 2] = unit[j].z, w[4 * j + 3] = unit[j].w;
+    const uint32_t d = reinterpret_cast<uintptr_t>(row + c0) & 15;
+    const bool last = lane == LANES - 1;
+    const uint4 e = extra;
+    const uint32_t after[4] = {e.x, e.y, e.z, e.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t n = __shfl_down_sync(0xffffffffu, w[j], 1, LANES);
+      w[4 * kUnits + j] = last ? after[j] : n;
+    }
+#pragma unroll
+    for (int i = 0; i < 4 * kUnits + 2; ++i) w[i] = (d & 8) ? w[i + 2] : w[i];
+#pragma unroll
+    for (int i = 0; i < 4 * kUnits + 1; ++i) w[i] = (d & 4) ? w[i + 1] : w[i];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(__funnelshift_r(w[i], w[i + 1], (d & 2) * 8), T());
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+      }
+    }
+    drop_past(c0, cols, lane, v);
+  }
+};
+// What a lane of the quantising kernels loads ahead.
+template <bool VEC, int LANES, class T>
+struct Ahead8 {
+  std::conditional_t<VEC, Raw8<T>, Shifted8<LANES, T>> raw;
+  __device__ __forceinline__ void load(const T* row, int c0, int cols, int lane) {
+    if constexpr (VEC)
+      load_raw<true>(row, c0, cols, lane, raw);
+    else
+      raw.load(row, c0, cols, lane);
+  }
+  __device__ __forceinline__ void get(const T* row, int c0, int cols, int lane, float (&v)[8]) const {
+    if constexpr (VEC)
+      raw.get(v);
+    else
+      raw.get(row, c0, cols, lane, v);
+  }
+};
 template <bool VEC, class T>
 __device__ __forceinline__ void load_cols(const T* row, int c0, int cols, int lane, float (&v)[8]) {
   if (VEC && c0 + lane * 8 + 8 <= cols) {
@@ -200,12 +297,12 @@ __device__ __forceinline__ void store_cols(T* row, int c0, int cols, int lane, c
 }
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int lane, const float (&v)[8],
-                                            float inv) {
+                                            float inv, bool aligned = true) {
   const float2 f = make_float2(inv, inv);
   const float2 a = __fmul2_rn(make_float2(v[0], v[1]), f), b = __fmul2_rn(make_float2(v[2], v[3]), f);
   const float2 c = __fmul2_rn(make_float2(v[4], v[5]), f), d = __fmul2_rn(make_float2(v[6], v[7]), f);
   const uint32_t lo = e4m3x4(a.x, a.y, b.x, b.y), hi = e4m3x4(c.x, c.y, d.x, d.y);
-  if (VEC && c0 + lane * 8 + 8 <= cols) {
+  if (VEC && aligned && c0 + lane * 8 + 8 <= cols) {
     *reinterpret_cast<uint2*>(row + c0 + lane * 8) = make_uint2(lo, hi);
     return;
   }

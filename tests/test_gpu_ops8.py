@@ -97,6 +97,32 @@ def test_quant8(lb, kind, br, rows, cols, pad, shift):
     assert canary_kept(buf, rows, cols)
 
 
+def in_nan(x, pitch, shift):
+    """x as a view of a buffer of NaN: rows `pitch` apart, the first `shift` values in."""
+    buf = torch.full((x.shape[0] * pitch + shift + x.shape[1],), math.nan, dtype=x.dtype, device="cuda")
+    view = buf.as_strided(x.shape, (pitch, 1), shift)
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("br", [1, 128])
+@pytest.mark.parametrize("rows,cols", [(5, 1), (9, 8), (70, 100), (131, 127), (33, 129), (40, 249), (64, 255), (300, 256),
+                                       (37, 263), (129, 600)])
+def test_quant8_rows_at_any_offset(lb, kind, br, rows, cols):
+    """The same bits wherever rows start; what stands around them is neither read as theirs nor written."""
+    x = rnd((rows, cols), 31 * rows + cols, TYPES[kind])
+    q0, s0, _ = out8(rows, cols, br)
+    lb.quant8(x.contiguous() if cols % 8 == 0 else in_nan(x, cols + -cols % 8, 0), q0, s0, block_rows=br)
+    for shift in range(8):
+        for pitch in (cols, cols + 1, cols + 3 + -cols % 8):
+            q, s, buf = out8(rows, cols, br, pitch=cols + shift)
+            lb.quant8(in_nan(x, pitch, shift), q, s, block_rows=br)
+            torch.cuda.synchronize()
+            assert torch.equal(q.view(torch.uint8), q0.view(torch.uint8)) and torch.equal(s, s0), (shift, pitch)
+            assert canary_kept(buf, rows, cols)
+
+
 @pytest.mark.parametrize("kind", list(TYPES))
 @pytest.mark.parametrize("br", [1, 128])
 def test_quant8_special_values(lb, kind, br):
@@ -181,6 +207,27 @@ def test_add_norm_quant8(lb, xt, rt, rows, cols, pad, shift):
     lb.add_norm_quant8(x, None, gamma, None, q2, s2)
     torch.cuda.synchronize()
     check_norm(q2, s2, true_norm(x.double(), gamma, 0.0))
+
+
+@pytest.mark.parametrize("xt,rt", [("f32", "f32"), ("f16", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("rows,cols", [(3, 5), (70, 255), (33, 301), (20, 511), (41, 700), (7, 2050), (5, 5001), (3, 17003)])
+def test_add_norm_quant8_padding_is_not_read(lb, xt, rt, rows, cols):
+    """NaN behind the rows, and rows that start on no boundary, change nothing."""
+    x, r = rnd((rows, cols), cols, TYPES[xt]), rnd((rows, cols), cols + 1, TYPES[rt])
+    gamma = rnd((1, cols), 7)[0]
+    for shift, extra in ((0, -cols % 8), (3, 0)):
+        outs = []
+        for fill in (in_nan, lambda t, pitch, at: torch.nan_to_num_(in_nan(t, pitch, at)._base, nan=2.0).as_strided(
+                t.shape, (pitch, 1), at)):
+            xv, rv = fill(x, cols + extra, shift), fill(r, cols + extra, shift)
+            q, s, buf = out8(rows, cols)
+            lb.add_norm_quant8(xv, rv, gamma, rv, q, s)  # the sum over its residual
+            torch.cuda.synchronize()
+            assert canary_kept(buf, rows, cols) and torch.isfinite(s).all()
+            outs.append((q.view(torch.uint8).clone(), s, rv.clone()))
+            assert rv._base[:shift].isnan().all() if fill is in_nan else (rv._base[:shift] == 2.0).all()
+        assert all(torch.equal(a, b) for a, b in zip(*outs))
+        assert torch.equal(outs[0][2], (x.float() + r.float()).to(TYPES[rt]))
 
 
 def test_add_norm_quant8_matches_the_trunk_norm(lb):
