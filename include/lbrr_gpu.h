@@ -336,8 +336,10 @@ int lbrr_op_feed_forward_noalloc(const uint16_t* h16, const uint16_t* w1_16, con
  * scales[(c / 128) * lds + r / block_rows].  It stands for q * scale.  A block's
  * scale is max|v| / 448 (at least 2^-126) and its codes are v / scale rounded
  * to nearest even; a block that holds an infinity or a NaN has scale NaN and
- * NaN codes throughout.  Bytes between the last column and the next row are
- * neither read nor written; they may hold anything.
+ * NaN codes throughout.  Bytes between the last column and the next row may hold
+ * anything: no result depends on them and they are not written.  (Loads are whole
+ * 16-byte units that hold a value of the row, so up to 15 bytes beside a row may be
+ * read and dropped.)
  *
  * All four are asynchronous on `stream` (NULL: the legacy default stream) of
  * the current device, on which every pointer must lie; none allocates, except

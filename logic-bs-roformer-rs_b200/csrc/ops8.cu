@@ -97,6 +97,8 @@ extern "C" int lbrr_op_add_norm_quant8(const void* x, int32_t x_type, int64_t ld
   if (!gamma || reinterpret_cast<uintptr_t>(gamma) % 4 != 0) return bad(op, "bad gamma");
   if (!ok_matrix(q, ldq, cols, 1)) return bad(op, "bad q");
   if (!ok_matrix(scales, lds, rows, 4)) return bad(op, "bad scales");
+  if (y && ((y == resid && rows > 1 && ldy != ldr) || (y == x && (resid_type != x_type || (rows > 1 && ldy != ldx)))))
+    return bad(op, "y in place needs the input's type and distance between rows");
   AddNorm8 a{};
   a.x = x;
   a.x_type = static_cast<Elem>(x_type);
@@ -147,6 +149,7 @@ extern "C" int lbrr_op_gemm8(const uint8_t* a, int64_t lda, const float* a_scale
   if (int rc = check_product(op, a, lda, a_scales, ldas, w, ldw, w_scales, ldws, bias, m, n, k)) return rc;
   if (!ok_matrix(out, ldo, n, size_of(out_type))) return bad(op, "bad out");
   if (resid && !ok_matrix(resid, ldr, n, size_of(out_type))) return bad(op, "bad resid");
+  if (resid == out && m > 1 && ldr != ldo) return bad(op, "out in place needs resid's distance between rows");
   Gemm8 g = product(a, lda, a_scales, ldas, w, ldw, w_scales, ldws, bias, m, n, k);
   g.resid = resid;
   g.ldr = ldr;

@@ -49,6 +49,17 @@ def test_add_norm_quant8(change, word):
     refused(lbrr.lib().lbrr_op_add_norm_quant8(*{**NORM, **change}.values()), "lbrr_op_add_norm_quant8", word)
 
 
+@pytest.mark.parametrize("change", [
+    dict(), dict(x=2 * P, ldr=512), dict(x_type=F32, resid=2 * P, ldx=512), dict(x_type=F32, resid=2 * P, ldy=512)])
+def test_add_norm_quant8_in_place_needs_the_same_rows(change):
+    """y at x's or resid's address with another type or another distance between rows."""
+    refused(lbrr.lib().lbrr_op_add_norm_quant8(*{**NORM, **change}.values()), "lbrr_op_add_norm_quant8", "in place")
+
+
+def test_gemm8_in_place_needs_the_same_rows():
+    refused(lbrr.lib().lbrr_op_gemm8(*{**GEMM, "ldo": 208}.values()), "lbrr_op_gemm8", "in place")
+
+
 GEMM = dict(a=P, lda=256, a_scales=P, ldas=8, w=P, ldw=256, w_scales=P, ldws=2, bias=P, resid=P, ldr=200, out=P,
             out_type=F16, ldo=200, m=8, n=200, k=250, stream=None)
 GELU = dict(a=P, lda=256, a_scales=P, ldas=8, w=P, ldw=256, w_scales=P, ldws=2, bias=P, q=P, ldq=200, scales=P, lds=8,
