@@ -117,6 +117,28 @@ __device__ __forceinline__ uint32_t swz(int r, int o) {
   return static_cast<uint32_t>(r * 128 + ((((o >> 4) ^ (r & 7)) << 4) | (o & 15)));
 }
 
+// Rows R0, R0 + DR, ... of a whole block between a buffer and global memory in
+// 4-byte words, `at` being this lane's word of row R0.  Two warps per scheduler
+// hide little latency, so what counts is instructions per row: no predicates, one
+// addition per address (3500 x 4618 x 71 fp32:
+// 48 -> 29 us, 20 where rows are aligned).
+template <int R0, int DR>
+__device__ __forceinline__ void load_words(uint8_t* buf, uintptr_t at, int64_t step, int lane) {
+#pragma unroll 8
+  for (int r = R0; r < 32; r += DR, at += step)
+    cp_async4(buf + swz(r, lane * 4), reinterpret_cast<const void*>(at), true);
+}
+// HALF: the rows are halves that start between words; word j of a row holds columns 2j - 1 and 2j.
+template <int R0, int DR, bool HALF>
+__device__ __forceinline__ void store_words(const uint8_t* buf, uintptr_t at, int64_t step, int lane) {
+#pragma unroll 8
+  for (int r = R0; r < 32; r += DR, at += step) {
+    uint32_t w = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
+    if (HALF) w = __funnelshift_l(__shfl_up_sync(0xffffffffu, w, 1), w, 16);
+    if (!HALF || lane > 0) *reinterpret_cast<uint32_t*>(at) = w;
+  }
+}
+
 // One 32-row block of up to 128 bytes per row from global memory to a buffer,
 // asynchronously.  Rows on 16-byte boundaries and whole: 16 bytes a copy.
 // Otherwise 4-byte words: rows of halves that start between words come with the
@@ -135,13 +157,24 @@ __device__ __forceinline__ void load_block(uint8_t* buf, uint32_t* tail, const T
     }
     return;
   }
+  if (rows >= 32 && cols >= E) {
+    const uintptr_t word = ~uintptr_t(3), at = reinterpret_cast<uintptr_t>(src);
+    const int64_t step = ld * static_cast<int64_t>(sizeof(T));
+    if ((step & 3) == 0) {
+      load_words<0, 1>(buf, (at & word) + lane * 4, step, lane);
+    } else {  // every other row starts between words
+      load_words<0, 2>(buf, (at & word) + lane * 4, 2 * step, lane);
+      load_words<1, 2>(buf, ((at + step) & word) + lane * 4, 2 * step, lane);
+    }
+  } else {
 #pragma unroll 4
-  for (int r = 0; r < 32; ++r) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(src + r * ld);
-    const int half = (at & 2) != 0;  // never for 32-bit values
-    const int first = lane * (4 / static_cast<int>(sizeof(T))) - half;
-    if (r < rows && first < cols)
-      cp_async4(buf + swz(r, lane * 4), reinterpret_cast<const void*>((at & ~uintptr_t(3)) + lane * 4), true);
+    for (int r = 0; r < 32; ++r) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(src + r * ld);
+      const int half = (at & 2) != 0;  // never for 32-bit values
+      const int first = lane * (4 / static_cast<int>(sizeof(T))) - half;
+      if (r < rows && first < cols)
+        cp_async4(buf + swz(r, lane * 4), reinterpret_cast<const void*>((at & ~uintptr_t(3)) + lane * 4), true);
+    }
   }
   if (sizeof(T) == 2 && lane < rows && cols >= E) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(src + lane * ld);
@@ -156,7 +189,12 @@ __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t 
   cols = min(cols, E);
   auto value = [&](int r, int c) { return *reinterpret_cast<const T*>(buf + swz(r, c * static_cast<int>(sizeof(T)))); };
   const uintptr_t off = reinterpret_cast<uintptr_t>(dst) | (static_cast<uintptr_t>(ld) * sizeof(T));
-  if ((off & 3) == 0) {
+  const bool whole = rows >= 32 && cols == E && sizeof(T) > 1;
+  const int64_t step = ld * static_cast<int64_t>(sizeof(T));
+  const uintptr_t at = reinterpret_cast<uintptr_t>(dst) + lane * 4;
+  if (whole && (off & 3) == 0) {
+    store_words<0, 1, false>(buf, at, step, lane);
+  } else if ((off & 3) == 0) {
     const int words = cols / P;
 #pragma unroll 8
     for (int r = 0; r < 32; ++r)
@@ -165,15 +203,27 @@ __device__ __forceinline__ void store_block(const uint8_t* buf, T* dst, int64_t 
     for (int c = words * P; c < cols; ++c)
       if (lane < rows) dst[lane * ld + c] = value(lane, c);
   } else if (sizeof(T) == 2) {
-    // rows that start between words: word j of such a row holds columns 2j - 1 and 2j
+    // rows that start between words
+    if (whole) {
+      if ((step & 3) == 0) {
+        store_words<0, 1, true>(buf, at - 2, step, lane);
+      } else if ((at & 2) == 0) {
+        store_words<0, 2, false>(buf, at, 2 * step, lane);
+        store_words<1, 2, true>(buf, at + step - 2, 2 * step, lane);
+      } else {
+        store_words<0, 2, true>(buf, at - 2, 2 * step, lane);
+        store_words<1, 2, false>(buf, at + step, 2 * step, lane);
+      }
+    } else {
 #pragma unroll 8
-    for (int r = 0; r < 32; ++r) {
-      T* row = dst + r * ld;
-      const int half = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1, c = 2 * lane - half;
-      const uint32_t own = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
-      const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
-      if (r < rows && c >= 0 && c + 1 < cols)
-        *reinterpret_cast<uint32_t*>(row + c) = __funnelshift_l(before, own, half * 16);
+      for (int r = 0; r < 32; ++r) {
+        T* row = dst + r * ld;
+        const int half = static_cast<int>(reinterpret_cast<uintptr_t>(row) >> 1) & 1, c = 2 * lane - half;
+        const uint32_t own = *reinterpret_cast<const uint32_t*>(buf + swz(r, lane * 4));
+        const uint32_t before = __shfl_up_sync(0xffffffffu, own, 1);
+        if (r < rows && c >= 0 && c + 1 < cols)
+          *reinterpret_cast<uint32_t*>(row + c) = __funnelshift_l(before, own, half * 16);
+      }
     }
     if (lane < rows) {
       T* row = dst + lane * ld;

@@ -356,6 +356,32 @@ def test_gemm8_gelu_quant8(lb, m, n, k, with_bias):
     assert canary_kept(buf, m, n)
 
 
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("m,n,k", [(4097, 333, 200), (4130, 262, 70), (300, 333, 200), (33, 70, 300)])
+def test_gemm8_rows_at_any_offset(lb, kind, m, n, k):
+    """The same bits wherever the rows of the output and the residual start, and nothing beside them is written."""
+    dt = TYPES[kind]
+    a, sa, _ = out8(m, k)
+    w, sw, _ = out8(n, k, 128)
+    lb.quant8(rnd((m, k), 1), a, sa)
+    lb.quant8(rnd((n, k), 2, scale=k ** -0.5), w, sw, 128)
+    bias, r = rnd((1, n), 3)[0].contiguous(), rnd((m, n), 4, dt)
+    out = {}
+    for with_resid in (False, True):
+        out[with_resid] = torch.empty(m, n + -n % 8, dtype=dt, device="cuda")[:, :n]
+        lb.gemm8(a, sa, w, sw, out[with_resid], bias=bias, resid=in_nan(r, n + -n % 8, 0) if with_resid else None)
+    for shift in range(4):
+        for pitch in (n, n + 1, n + 2):
+            for rp, rs in ((None, 0), (n, 0), (n, 1), (n + 1, 0), (n + 1, 3)):
+                buf = torch.full((m * pitch + shift + 16,), 5.0, dtype=dt, device="cuda")
+                view = buf.as_strided((m, n), (pitch, 1), shift)
+                lb.gemm8(a, sa, w, sw, view, bias=bias, resid=None if rp is None else in_nan(r, rp, rs))
+                torch.cuda.synchronize()
+                assert torch.equal(view, out[rp is not None]), (shift, pitch, rp, rs)
+                view.fill_(5.0)
+                assert (buf == 5.0).all()
+
+
 @pytest.mark.parametrize("m,n,k", [(5, 200, 300), (300, 520, 1000), (4097, 130, 130), (9000, 200, 300)])
 def test_gemm8_adds_into_its_residual(lb, m, n, k):
     a, sa, a64 = operand(lb, m, k, 1, 1)
