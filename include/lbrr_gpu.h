@@ -335,7 +335,9 @@ int lbrr_op_feed_forward_noalloc(const uint16_t* h16, const uint16_t* w1_16, con
  * 128 rows (weights), stored by column block: the scale of q[r][c] is
  * scales[(c / 128) * lds + r / block_rows].  It stands for q * scale.  A block's
  * scale is max|v| / 448 (at least 2^-126) and its codes are v / scale rounded
- * to nearest even; a block that holds an infinity or a NaN has scale NaN and
+ * to nearest even: the fp32 quotient where v is the caller's (lbrr_op_quant8), the
+ * product with 1 / scale, within 2 ulp of it, where v is a norm or a GELU that the
+ * call forms; a block that holds an infinity or a NaN has scale NaN and
  * NaN codes throughout.  Bytes between the last column and the next row may hold
  * anything: no result depends on them and they are not written.  (Loads are whole
  * 16-byte units that hold a value of the row, so up to 15 bytes beside a row may be

@@ -21,15 +21,20 @@ namespace lbrr {
 // columns (16 lanes per block) at a time and has the next ones' loads in flight
 // meanwhile; eight warps cover 32 rows, so the scales of a block column leave
 // as whole sectors.  Unaligned rows (Shifted8) leave no registers for the loads
-// ahead: 71362 x 257 fp32 45 us, 53 with them; 37889 x 588 bf16 32 and 33.
+// ahead (at four blocks per SM: 71362 x 257 fp32 45 us, 53 with them; 37889 x 588
+// bf16 32 and 33).
 // ---------------------------------------------------------------------------
 constexpr int kRows8 = 4;
 constexpr int kWarps8 = 8;
-constexpr int kBlocksPerSm8 = 4;
+// Blocks per SM: four where 64 registers a thread are enough, three otherwise
+// (four, with spills: 71362 x 512 fp32 40 us and 30, 300000 x 64 fp16 22.5 and
+// 20.7, 37889 x 588 bf16 32.6 and 27.5, 71362 x 257 fp16 37 and 32).
+template <class T, bool VEC, bool NARROW>
+constexpr int kBlocksPerSm8 = VEC && !NARROW && sizeof(T) == 2 ? 4 : 3;
 
 // NARROW (up to 128 columns): the two halves of a warp take rows of their own.
 template <class T, bool VEC, bool NARROW>
-__global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
+__global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8<T, VEC, NARROW>)
     quant_rows_kernel(const T* __restrict__ x, int64_t ldx, int rows, int cols, uint8_t* __restrict__ q, int64_t ldq,
                       float* __restrict__ scales, int64_t lds, bool q_aligned) {
   constexpr int kPerWarp = NARROW ? 2 * kRows8 : kRows8;  // rows
@@ -64,12 +69,24 @@ __global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8)
     }
     if (kAhead) fetch(r0 + step);
     const Scales8<kRows8> sc = half_warp_scales<kRows8>(top, lane);
+    const Quotient8 own_quotient = quotient8(sc.own);
+    if (__any_sync(0xffffffffu, sc.own.s > kHugeScale8)) {
+      const float own_down = sc.own.s > kHugeScale8 ? kHugeDown8 : 1.0f;
 #pragma unroll
-    for (int i = 0; i < kRows8; ++i)
+      for (int i = 0; i < kRows8; ++i) {
+        const float down = sc.of(own_down, i, lane);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= down;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows8; ++i) {
+      const Quotient8 quotient{sc.of(own_quotient.hi, i, lane), sc.of(own_quotient.lo, i, lane)};
       if (row_of(r0, i) < rows)
-        store_codes<true>(q + static_cast<int64_t>(row_of(r0, i)) * ldq, c0, cols, at, v[i], sc.inv[i], VEC || q_aligned);
+        store_codes<true>(q + static_cast<int64_t>(row_of(r0, i)) * ldq, c0, cols, at, v[i], quotient, VEC || q_aligned);
+    }
     const int own = row_of(r0, sc.own_block), kb = NARROW ? 0 : blockIdx.y * 2 + half;
-    if (sc.writer && own < rows && kb * kBlock8 < cols) scales[kb * lds + own] = sc.own;
+    if (sc.writer && own < rows && kb * kBlock8 < cols) scales[kb * lds + own] = sc.own.s;
   }
 }
 
@@ -121,10 +138,17 @@ __global__ void __launch_bounds__(kTileThreads8, 2)
     __syncthreads();  // one per block: the next block writes the other half of `part`
     top = __reduce_max_sync(0xffffffffu, part[it][lane & (kTileThreads8 / 32 - 1)]);
     const Scale8 s = scale8(top);
+    const Quotient8 quotient = quotient8(s);
+    if (s.s > kHugeScale8) {  // the same for every thread
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] *= kHugeDown8;
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int r = r0 + i * kStep;
-      if (r < rows) store_codes<true>(q + static_cast<int64_t>(r) * ldq, bx * kBlock8, cols, l16, v[i], s.inv, VEC || q_aligned);
+      if (r < rows) store_codes<true>(q + static_cast<int64_t>(r) * ldq, bx * kBlock8, cols, l16, v[i], quotient, VEC || q_aligned);
     }
     if (threadIdx.x == 0) scales[bx * lds + by] = s.s;
     if (!kAhead) break;
@@ -145,7 +169,9 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
     const bool narrow = cols <= kBlock8;
     const int per_block = kWarps8 * kRows8 * (narrow ? 2 : 1);
     const int groups = (rows + per_block - 1) / per_block, chunks = (cols + 2 * kBlock8 - 1) / (2 * kBlock8);
-    const int resident = std::max(1, kBlocksPerSm8 * 148 / chunks);  // blocks per column chunk that run at one time
+    const int per_sm = vec ? (narrow ? kBlocksPerSm8<T, true, true> : kBlocksPerSm8<T, true, false>)
+                           : (narrow ? kBlocksPerSm8<T, false, true> : kBlocksPerSm8<T, false, false>);
+    const int resident = std::max(1, per_sm * 148 / chunks);  // blocks per column chunk that run at one time
     const dim3 grid(std::min(groups, resident), chunks);
     auto k = vec ? (narrow ? quant_rows_kernel<T, true, true> : quant_rows_kernel<T, true, false>)
                  : (narrow ? quant_rows_kernel<T, false, true> : quant_rows_kernel<T, false, false>);
@@ -304,10 +330,12 @@ __global__ void __launch_bounds__(THREADS, THREADS == 512 ? 2 : 1)
       tops[i] = top_of(v[i]);
     }
     const Scales8<C> sc = half_warp_scales<C>(tops, lane);
+    float inverse[C];
+    inverses(sc, lane, inverse);
 #pragma unroll
-    for (int i = 0; i < C; ++i) store_codes<VEC>(q + row * ldq, (wr + i * warps) * 256, cols, lane, v[i], sc.inv[i]);
+    for (int i = 0; i < C; ++i) store_codes<VEC>(q + row * ldq, (wr + i * warps) * 256, cols, lane, v[i], inverse[i]);
     const int kb = (wr + sc.own_block * warps) * 2 + (lane >> 4);
-    if (sc.writer && kb * kBlock8 < cols) scales[kb * lds + row] = sc.own;
+    if (sc.writer && kb * kBlock8 < cols) scales[kb * lds + row] = sc.own.s;
     if (!LOOP || row + step >= rows) break;
   }
 }

@@ -3,10 +3,13 @@
 // of the 8-bit matrix product.
 //
 // A block with largest magnitude t is held as q = e4m3(v / s), s = t / 448
-// (448: the largest finite e4m3 value).  Two roundings are choices: v / s is
-// computed as v * (1 / s) (within 2 ulp of 32 bits, far below e4m3's half
-// step of 2^-4), and q is rounded to nearest even with saturation, so the
-// block's largest value, which may land an ulp above 448, stays 448.  s is at
+// (448: the largest finite e4m3 value).  Where the values are a caller's, v / s
+// is the fp32 quotient (`Quotient8`): 11-bit inputs land on e4m3's rounding
+// borders often, and a quotient an ulp off falls on the wrong side of them (six
+// codes in 10^5 of fp16 rows).  Where the values are a kernel's own, with
+// several roundings in them, it is v * (1 / s), within 2 ulp of 32 bits.  q is
+// rounded to nearest even with saturation, so the block's largest value, which
+// may land an ulp above 448, stays 448.  s is at
 // least 2^-126, so 1 / s is finite and a block of zeros is held as zeros.  A
 // block that holds an infinity or a NaN gets scale NaN and NaN codes (0x7f):
 // nothing in it could be told apart.
@@ -46,12 +49,36 @@ __device__ __forceinline__ Scale8 scale8(uint32_t top) {
   if (top >= 0x7f800000u) {
     r.s = r.inv = __uint_as_float(0x7fffffffu);
   } else {
-    // t / 448, correctly rounded: the product with 1 / 448, corrected once by its remainder (exact in an FMA)
+    // t / 448, rounded once: the product with the reciprocal, corrected by its remainder, which one FMA forms
+    // exactly (Markstein's division, IBM J. Res. Dev. 34, 1990)
     const float t = __uint_as_float(top), c = 1.0f / kE4m3Max;
     const float q = t * c;
     r.s = fmaxf(fmaf(fmaf(-q, kE4m3Max, t), c, q), kMinScale8);
     asm("rcp.approx.f32 %0, %1;" : "=f"(r.inv) : "f"(r.s));  // within 1 ulp
   }
+  return r;
+}
+
+// Division of a block's values by its scale: v hi + v lo in one FMA after a
+// product, hi + lo = 1 / s to 2^-44 (a sum of two fp32 numbers, Dekker, Numer.
+// Math. 18, 1971; lo is hi's Newton correction), so the result is v / s rounded
+// once, the fp32 quotient but for quotients that close to the middle between two
+// fp32 numbers.  hi is taken a little low: lo is then positive, and a zero keeps
+// its sign.  lo would leave the normal range beside a huge s, so those blocks are
+// divided as (2^-64 v) / (2^-64 s).
+constexpr float kHugeScale8 = 0x1p80f, kHugeDown8 = 0x1p-64f;
+struct Quotient8 {
+  float hi, lo;
+  __device__ __forceinline__ float2 of(float2 v) const {
+    return __ffma2_rn(v, make_float2(hi, hi), __fmul2_rn(v, make_float2(lo, lo)));
+  }
+};
+__device__ __forceinline__ Quotient8 quotient8(Scale8 by) {
+  const bool huge = by.s > kHugeScale8;
+  const float s = huge ? by.s * kHugeDown8 : by.s;
+  Quotient8 r;
+  r.hi = (huge ? by.inv * (1.0f / kHugeDown8) : by.inv) * (1.0f - 0x1p-22f);
+  r.lo = fmaf(-s, r.hi, 1.0f) * r.hi;
   return r;
 }
 
@@ -295,22 +322,31 @@ __device__ __forceinline__ void store_cols(T* row, int c0, int cols, int lane, c
     if (c < cols) row[c] = from_f32<T>(v[j]);
   }
 }
-template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int lane, const float (&v)[8],
-                                            float inv, bool aligned = true) {
+// Eight codes, four to a word.
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], float inv) {
   const float2 f = make_float2(inv, inv);
   const float2 a = __fmul2_rn(make_float2(v[0], v[1]), f), b = __fmul2_rn(make_float2(v[2], v[3]), f);
   const float2 c = __fmul2_rn(make_float2(v[4], v[5]), f), d = __fmul2_rn(make_float2(v[6], v[7]), f);
-  const uint32_t lo = e4m3x4(a.x, a.y, b.x, b.y), hi = e4m3x4(c.x, c.y, d.x, d.y);
+  return make_uint2(e4m3x4(a.x, a.y, b.x, b.y), e4m3x4(c.x, c.y, d.x, d.y));
+}
+__device__ __forceinline__ uint2 codes8(const float (&v)[8], const Quotient8& by) {
+  const float2 a = by.of(make_float2(v[0], v[1])), b = by.of(make_float2(v[2], v[3]));
+  const float2 c = by.of(make_float2(v[4], v[5])), d = by.of(make_float2(v[6], v[7]));
+  return make_uint2(e4m3x4(a.x, a.y, b.x, b.y), e4m3x4(c.x, c.y, d.x, d.y));
+}
+template <bool VEC, class By>
+__device__ __forceinline__ void store_codes(uint8_t* row, int c0, int cols, int lane, const float (&v)[8],
+                                            const By& by, bool aligned = true) {
+  const uint2 q = codes8(v, by);
   if (VEC && aligned && c0 + lane * 8 + 8 <= cols) {
-    *reinterpret_cast<uint2*>(row + c0 + lane * 8) = make_uint2(lo, hi);
+    *reinterpret_cast<uint2*>(row + c0 + lane * 8) = q;
     return;
   }
   if (VEC && c0 + lane * 8 >= cols) return;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int at = c0 + lane_col<VEC>(lane, j);
-    if (at < cols) row[at] = static_cast<uint8_t>((j < 4 ? lo >> (8 * j) : hi >> (8 * (j - 4))) & 0xffu);
+    if (at < cols) row[at] = static_cast<uint8_t>((j < 4 ? q.x >> (8 * j) : q.y >> (8 * (j - 4))) & 0xffu);
   }
 }
 // Largest magnitude of eight values, as bits (NaN above all).
@@ -319,17 +355,20 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[8]) {
   return __float_as_uint(max_mag3(max_mag3(a, v[2], v[3]), max_mag3(b, v[6], v[7]), 0.0f));
 }
 
-// The scales of R blocks (1, 2 or 4) that 16 lanes hold together: from every
-// lane's own maxima, each block's inverse scale in every lane, and its scale in
-// lane `own_block`'s lanes.  The exchange halves the number of blocks a lane
-// follows until it has one, so R blocks take R + 3 shuffles (and R to hand the
-// inverses back), not 4 R, and one scale per lane is computed, not R.
+// The scales of R blocks (1, 2 or 4) that 16 lanes hold together, from every
+// lane's own maxima.  The exchange halves the number of blocks a lane follows
+// until it has one, so R blocks take R + 3 shuffles (and one to hand a number on),
+// not 4 R, and one scale per lane is computed, not R.  Every lane of the warp
+// calls these.
 template <int R>
 struct Scales8 {
-  float inv[R];
-  float own;       // the scale of block own_block
+  Scale8 own;      // of block own_block
   int own_block;
   bool writer;     // one lane per block
+
+  __device__ __forceinline__ float of(float own_number, int block, int lane) const {
+    return R == 1 ? own_number : __shfl_sync(0xffffffffu, own_number, (lane & 16) | (block * (16 / R)));
+  }
 };
 template <int R>
 __device__ __forceinline__ Scales8<R> half_warp_scales(const uint32_t (&top)[R], int lane) {
@@ -357,11 +396,14 @@ __device__ __forceinline__ Scales8<R> half_warp_scales(const uint32_t (&top)[R],
   }
   k = max(k, __shfl_xor_sync(all, k, 2));
   k = max(k, __shfl_xor_sync(all, k, 1));
-  const Scale8 s = scale8(k);
-  r.own = s.s;
-#pragma unroll
-  for (int i = 0; i < R; ++i) r.inv[i] = R == 1 ? s.inv : __shfl_sync(all, s.inv, (lane & 16) | (i * (16 / R)));
+  r.own = scale8(k);
   return r;
+}
+// Every block's inverse scale in every lane.
+template <int R>
+__device__ __forceinline__ void inverses(const Scales8<R>& sc, int lane, float (&inv)[R]) {
+#pragma unroll
+  for (int i = 0; i < R; ++i) inv[i] = sc.of(sc.own.inv, i, lane);
 }
 
 }  // namespace lbrr
