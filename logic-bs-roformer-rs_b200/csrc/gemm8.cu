@@ -45,6 +45,7 @@
 #include "gelu8.cuh"
 #include "gemm8_few.cuh"
 #include "quant8.cuh"
+#include "ring.h"
 
 namespace lbrr {
 
@@ -323,6 +324,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
           tma_load_2d_pair(sa + kABytes8, &tmW, bar, kb * kK8, w_row);
         }
       }
+      // The commits that free the stages arrive on both CTAs' barriers by themselves, and the final cluster barrier does
+      // not wait for them: the last ones have arrived before either CTA may go.
+      ok = ok && drain_ring<kStages8>(c, [&](int s, uint32_t parity) {
+             return mbar_wait(&empty[s], parity, abort_flag, status);
+           });
       if (!ok && rank == 0) {  // the pair's copies in flight land before its shared memory goes
         for (uint32_t i = c > kStages8 ? c - kStages8 : 0; i < c; ++i) {
           int none = 0;

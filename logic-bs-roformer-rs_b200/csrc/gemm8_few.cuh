@@ -27,6 +27,7 @@
 #include "cp_async.cuh"
 #include "gelu8.cuh"
 #include "quant8.cuh"
+#include "ring.h"
 
 namespace lbrr {
 
@@ -240,6 +241,10 @@ __global__ void __launch_bounds__(FewLayout<NT>::kThreads, 2)
         if (!(ok = mbar_wait(&empty[c % L::kStages], ((c / L::kStages) & 1) ^ 1u, abort_flag, status))) break;
         load(c);
       }
+      // the commits that free the stages have arrived before the block may go
+      ok = ok && drain_ring<L::kStages>(blocks, [&](int s, uint32_t parity) {
+             return mbar_wait(&empty[s], parity, abort_flag, status);
+           });
       if (!ok) {  // the copies in flight land before the block's shared memory goes
         for (int i = c > L::kStages ? c - L::kStages : 0; i < c; ++i) {
           int none = 0;
