@@ -31,13 +31,15 @@
 // the totals' latency bound it.  71362 x 1536 x 256 to fp16 57 us (4.2 TB/s, 3950
 // cycles a tile: totals 1300, conversion and staging 950, stores 300-500, waits
 // 500), 71362 x 256 x 1024 with fp32 residual 52 us (4.3 TB/s; a CTA's 384 KB a
-// tile take 16.7 k of its 21 k cycles), 71362 x 1024 x 256 with GELU to 8 bits 54
-// us (5900 cycles a tile, 3000 of them GELU, whose MUFU part alone is 2070).
+// tile take 16.7 k of its 21 k cycles), 71362 x 1024 x 256 with GELU to 8 bits 61
+// us (about 6600 cycles a tile, 3700 of them GELU, whose MUFU part alone is 2070).
 // Tried and left out: one CTA per 128 x 256 tile (8192^3 662 us against 607 for
 // the pair at that time), a second issuing warp (the two accumulators' MMAs
 // interleave and end together: 675), 256 x 128 tiles with two sets of output
 // warps on alternate tiles (8192^3 696, 71362 x 1024 x 256 55), an L2 prefetch of
 // the residual (52 -> 60 us), the bias added with the conversions (57 -> 65 us).
+#include <math_constants.h>
+
 #include <atomic>
 
 #include "cp_async.cuh"
@@ -537,6 +539,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
           for (int i = 0; i < kPart8 / 2; ++i) {
             if (2 * i >= cols) acc[i].x = 0.0f;
             if (2 * i + 1 >= cols) acc[i].y = 0.0f;
+          }
+        }
+        // A row whose block holds nothing large needs the tail's own fit.  A large value is usually among the first
+        // columns; where a row of the warp has none there, all columns are looked at.  No row's bits depend on another.
+        float high = -CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < kPart8 / 8; ++i) high = max3(high, acc[i].x, acc[i].y);
+        if (__any_sync(0xffffffffu, high < kGelu8Large)) {
+          float low = 0.0f;
+#pragma unroll
+          for (int i = 0; i < kPart8 / 2; ++i) {
+            high = max3(high, acc[i].x, acc[i].y);
+            low = min3(low, acc[i].x, acc[i].y);
+          }
+          const bool tail = high < kGelu8Large && low < kGelu8Tail;
+          if (__any_sync(0xffffffffu, tail)) {
+            const float from = tail ? kGelu8Tail : -CUDART_INF_F;
+#pragma unroll
+            for (int i = 0; i < kPart8 / 2; ++i) acc[i] = before_gelu8(acc[i], from);
           }
         }
 #pragma unroll

@@ -129,6 +129,11 @@ __device__ __forceinline__ void few_rows(const FewParams& p, const float* in, in
     for (int i = 0; i < 4; ++i) h[i] += bias[i];
     const int64_t m = m0 + r;
     if constexpr (sizeof(T) == 1) {
+      if (__any_sync(0xffffffffu, fminf(min3(h[0], h[1], h[2]), h[3]) < kGelu8Tail)) {
+        const float2 a = before_gelu8(make_float2(h[0], h[1]), kGelu8Tail);
+        const float2 b = before_gelu8(make_float2(h[2], h[3]), kGelu8Tail);
+        h[0] = a.x, h[1] = a.y, h[2] = b.x, h[3] = b.y;
+      }
       const float2 a = gelu8(make_float2(h[0], h[1])), b = gelu8(make_float2(h[2], h[3]));
       uint32_t top = 0;
       if (0 < left) top = max(top, mag_bits(a.x));
