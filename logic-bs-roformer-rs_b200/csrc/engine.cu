@@ -1956,7 +1956,10 @@ int* lbrr::op_status(bool peek) {
   if (it != per_dev.end()) return it->second;
   if (peek) return nullptr;
   int* p = nullptr;
-  if (cudaMalloc(&p, 64 * sizeof(int)) != cudaSuccess) return nullptr;
+  if (cudaMalloc(&p, 64 * sizeof(int)) != cudaSuccess) {
+    cudaGetLastError();  // the caller reports it
+    return nullptr;
+  }
   cudaMemset(p, 0, 64 * sizeof(int));
   cudaDeviceSynchronize();
   per_dev[dev] = p;

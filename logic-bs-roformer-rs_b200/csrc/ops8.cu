@@ -14,6 +14,7 @@ int bad(const char* op, const std::string& what) {
 }
 int launched(const char* op, cudaError_t e) {
   if (e == cudaSuccess) return LBRR_OK;
+  cudaGetLastError();  // reported here: the next call's launch does not find it
   return lbrr_set_error_for_host(LBRR_ERR_CUDA, (std::string(op) + ": " + cudaGetErrorString(e)).c_str());
 }
 
@@ -51,11 +52,13 @@ int status_word(const char* op, cudaStream_t st, int** status) {
   *status = op_status(true);
   if (!*status) {
     cudaStreamCaptureStatus cs = cudaStreamCaptureStatusNone;
-    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone)
+    if (cudaStreamIsCapturing(st, &cs) != cudaSuccess || cs != cudaStreamCaptureStatusNone) {
+      cudaGetLastError();  // the default stream beside a blocking one's capture cannot be asked
       return lbrr_set_error_for_host(
           LBRR_ERR_STATE,
           (std::string(op) + ": call a per-op entry point once on this device before recording it into a graph")
               .c_str());
+    }
     *status = op_status();
   }
   if (!*status) return lbrr_set_error_for_host(LBRR_ERR_CUDA, "op status allocation failed");
