@@ -346,7 +346,7 @@ int lbrr_op_feed_forward_noalloc(const uint16_t* h16, const uint16_t* w1_16, con
  * All four are asynchronous on `stream` (NULL: the legacy default stream) of
  * the current device, on which every pointer must lie; none allocates, except
  * that the first product on a device allocates its status word (make that call
- * outside a graph capture; during one it is refused with LBRR_ERR_STATE).
+ * outside a capture of its stream; during one it is refused with LBRR_ERR_STATE).
  * Calls keep nothing between them and use no shared workspace, so any number
  * may run at once.  Distances between rows (ld*) count elements.  Except where
  * noted, outputs must not overlap inputs.  rows == 0 / m == 0 is no work.

@@ -1955,13 +1955,22 @@ int* lbrr::op_status(bool peek) {
   auto it = per_dev.find(dev);
   if (it != per_dev.end()) return it->second;
   if (peek) return nullptr;
+  // Captures under way on other streams are not this allocation's business: the calls below say so (relaxed mode), and
+  // the word is cleared on a stream of its own.
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
   int* p = nullptr;
-  if (cudaMalloc(&p, 64 * sizeof(int)) != cudaSuccess) {
+  cudaStream_t st = nullptr;
+  bool ok = cudaMalloc(&p, 64 * sizeof(int)) == cudaSuccess &&
+            cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking) == cudaSuccess;
+  ok = ok && cudaMemsetAsync(p, 0, 64 * sizeof(int), st) == cudaSuccess && cudaStreamSynchronize(st) == cudaSuccess;
+  if (st) cudaStreamDestroy(st);
+  if (!ok) {
+    if (p) cudaFree(p);
     cudaGetLastError();  // the caller reports it
-    return nullptr;
   }
-  cudaMemset(p, 0, 64 * sizeof(int));
-  cudaDeviceSynchronize();
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!ok) return nullptr;
   per_dev[dev] = p;
   return p;
 }

@@ -1,5 +1,6 @@
-"""What a refused or failed call of the 8-bit operators leaves behind: nothing, the next call does not report an earlier
-one's error.  Each case needs a process of its own, whose first product has not been called yet."""
+"""What a refused or failed call of the 8-bit operators leaves behind: nothing.  The next call does not report an earlier
+one's error, and captures under way elsewhere stay whole.  Each case needs a process of its own, whose first product has
+not been called yet."""
 import subprocess
 import sys
 from pathlib import Path
@@ -59,6 +60,20 @@ with c:
 assert c.rc == 0
 quantise()
 product(); right()
+""",
+    # the first product of the process while another stream is being captured: that capture is not its business
+    "first_product_beside_a_capture": """
+quantise(); torch.cuda.synchronize()
+other, y = torch.cuda.Stream(), torch.zeros(8, device="cuda")
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g, stream=other):
+    y.add_(1.0)
+    product()
+    y.add_(1.0)
+right()
+g.replay(); torch.cuda.synchronize()
+assert (y == 2.0).all()
 """,
     # a launch that fails on the host is reported once
     "failed_launch": """
