@@ -467,14 +467,19 @@ def _vector(t, name, n, dev):
 
 
 def _same_rows(name, t, ld, other_name, other, other_ld):
-    """Refuses an output that overlaps an input other than element for element."""
+    """Refuses an output that overlaps an input other than element for element.  Columns of one buffer beside each
+    other do not overlap."""
     a0, b0 = t.data_ptr(), other.data_ptr()
     if a0 == b0 and ld == other_ld and t.dtype == other.dtype:
         return
     rows, cols = t.shape
-    if a0 < b0 + other.element_size() * ((rows - 1) * other_ld + cols) and \
-            b0 < a0 + t.element_size() * ((rows - 1) * ld + cols):
-        _bad(f"{name} overlaps {other_name} without being the same tensor")
+    pitch, other_pitch = ld * t.element_size(), other_ld * other.element_size()
+    width, other_width = cols * t.element_size(), cols * other.element_size()
+    if a0 >= b0 + (rows - 1) * other_pitch + other_width or b0 >= a0 + (rows - 1) * pitch + width:
+        return
+    if rows > 1 and pitch == other_pitch and width <= (b0 - a0) % pitch <= pitch - other_width:
+        return
+    _bad(f"{name} overlaps {other_name} without being the same tensor")
 
 
 def _call8(dev, stream, fn, *args):
