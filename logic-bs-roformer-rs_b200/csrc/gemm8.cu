@@ -669,8 +669,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads8, 1)
   }
 }
 
-// Pairs that run at one time on the current device.
-static int resident_pairs(const void* kernel) {
+// Pairs of a kernel that run at one time on the current device.
+template <Out8 O, bool ODD>
+static int resident_pairs() {
   static std::atomic<int> known[64];
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
@@ -687,7 +688,7 @@ static int resident_pairs(const void* kernel) {
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+  if (cudaOccupancyMaxActiveClusters(&n, gemm8_kernel<O, ODD>, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
     n = sms / 2 > 0 ? sms / 2 : 1;
   }
@@ -710,7 +711,7 @@ static cudaError_t launch8(const CUtensorMap& ta, const CUtensorMap& tw, const C
   });
   if (e != cudaSuccess) return e;
   const int tiles = p.mt * p.nt;
-  const int pairs = resident_pairs(reinterpret_cast<const void*>(gemm8_kernel<O, ODD>));
+  const int pairs = resident_pairs<O, ODD>();
   count_launch();
   gemm8_kernel<O, ODD><<<2 * (tiles < pairs ? tiles : pairs), kThreads8, kSmem8, st>>>(ta, tw, to, p, status);
   return cudaGetLastError();
@@ -772,7 +773,7 @@ static cudaError_t gemm8_few(const Gemm8& g, int* status, cudaStream_t st) {
   const int64_t tiles = static_cast<int64_t>((g.n + 127) / 128) * ((g.m + nt - 1) / nt);
   // as many CTAs per tile as two per SM allow, each with a K-block at least
   p.lg = 0;
-  while ((1 << p.lg) < kFewMaxSplit && (tiles << (p.lg + 1)) <= 2 * 148 && (2 << p.lg) <= p.kb) ++p.lg;
+  while ((1 << p.lg) < kFewMaxSplit && (tiles << (p.lg + 1)) <= 2 * kSms && (2 << p.lg) <= p.kb) ++p.lg;
   p.split = 1 << p.lg;
   return nt == 16 ? launch_few<16>(p, status, st)
                   : nt == 32 ? launch_few<32>(p, status, st) : launch_few<64>(p, status, st);
@@ -783,7 +784,7 @@ static cudaError_t gemm8_few(const Gemm8& g, int* status, cudaStream_t st) {
 // against 512 x 4096 x 4096 24.5 (18.9), 1024 x 2048 x 2048 15.4 (12.7), 2294 x 1536 x 256 10.2 (7.1).
 cudaError_t gemm8(const Gemm8& g, int* status, cudaStream_t st) {
   const int64_t tiles = static_cast<int64_t>((g.m + 63) / 64) * ((g.n + 127) / 128);
-  return g.m <= 64 || tiles <= 148 ? gemm8_few(g, status, st) : gemm8_tiled(g, status, st);
+  return g.m <= 64 || tiles <= kSms ? gemm8_few(g, status, st) : gemm8_tiled(g, status, st);
 }
 
 }  // namespace lbrr

@@ -116,6 +116,7 @@ cudaError_t istft_back(const float2* c2r, const float* window, const float2* twi
 // and per row (or per 128 rows)
 enum class Elem { F32 = 0, F16 = 1, BF16 = 2 };
 constexpr int kNorm8MaxCols = 32768;
+constexpr int kSms = 148;  // of a B200: grids and choices of kernel are sized for it
 cudaError_t quant8(const void* x, Elem type, int64_t ldx, int rows, int cols, int block_rows, uint8_t* q, int64_t ldq,
                    float* scales, int64_t lds, cudaStream_t st);
 struct AddNorm8 {

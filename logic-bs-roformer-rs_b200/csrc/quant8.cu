@@ -171,7 +171,7 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
     const int groups = (rows + per_block - 1) / per_block, chunks = (cols + 2 * kBlock8 - 1) / (2 * kBlock8);
     const int per_sm = vec ? (narrow ? kBlocksPerSm8<T, true, true> : kBlocksPerSm8<T, true, false>)
                            : (narrow ? kBlocksPerSm8<T, false, true> : kBlocksPerSm8<T, false, false>);
-    const int resident = std::max(1, per_sm * 148 / chunks);  // blocks per column chunk that run at one time
+    const int resident = std::max(1, per_sm * kSms / chunks);  // blocks per column chunk that run at one time
     const dim3 grid(std::min(groups, resident), chunks);
     auto k = vec ? (narrow ? quant_rows_kernel<T, true, true> : quant_rows_kernel<T, true, false>)
                  : (narrow ? quant_rows_kernel<T, false, true> : quant_rows_kernel<T, false, false>);
@@ -180,7 +180,7 @@ static cudaError_t quant8_t(const void* xv, int64_t ldx, int rows, int cols, int
     const int blocks_x = (cols + kBlock8 - 1) / kBlock8;
     const int blocks = blocks_x * ((rows + kBlock8 - 1) / kBlock8);
     auto k = vec ? quant_tiles_kernel<T, true> : quant_tiles_kernel<T, false>;
-    k<<<vec && sizeof(T) == 2 ? std::min(blocks, 2 * 148) : blocks, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds,
+    k<<<vec && sizeof(T) == 2 ? std::min(blocks, 2 * kSms) : blocks, kTileThreads8, 0, st>>>(x, ldx, rows, cols, q, ldq, scales, lds,
                                                                                    q_aligned, blocks_x, blocks);
   }
   return cudaGetLastError();
@@ -372,7 +372,7 @@ static cudaError_t add_norm_quant8_t(const AddNorm8& a, cudaStream_t st) {
     // ahead), and unaligned rows, which load value by value (9402 x 1227 bf16: 26
     // and 37).
     const int warps = (chunks + 1) / 2, threads = warps * 32;
-    const int grid = vec && kAhead ? std::min(a.rows, 148 * (1024 / threads)) : a.rows;
+    const int grid = vec && kAhead ? std::min(a.rows, kSms * (1024 / threads)) : a.rows;
     if (threads <= 512)
       LBRR_LAUNCH(2, true, 512);
     else

@@ -134,13 +134,6 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
   v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
   v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
 }
-template <class T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
-  const uint4 a = *reinterpret_cast<const uint4*>(p);
-  const float2 f0 = unpack2(a.x, T()), f1 = unpack2(a.y, T()), f2 = unpack2(a.z, T()), f3 = unpack2(a.w, T());
-  v[0] = f0.x, v[1] = f0.y, v[2] = f1.x, v[3] = f1.y;
-  v[4] = f2.x, v[5] = f2.y, v[6] = f3.x, v[7] = f3.y;
-}
 __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
   reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
   reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -294,8 +287,8 @@ struct Ahead8 {
       raw.get(row, c0, cols, lane, v);
   }
 };
-template <bool VEC, class T>
-__device__ __forceinline__ void load_cols(const T* row, int c0, int cols, int lane, float (&v)[8]) {
+template <bool VEC>
+__device__ __forceinline__ void load_cols(const float* row, int c0, int cols, int lane, float (&v)[8]) {
   if (VEC && c0 + lane * 8 + 8 <= cols) {
     load8(row + c0 + lane * 8, v);
     return;
@@ -306,7 +299,7 @@ __device__ __forceinline__ void load_cols(const T* row, int c0, int cols, int la
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int c = c0 + lane_col<VEC>(lane, j);
-    if (c < cols) v[j] = to_f32(row[c]);
+    if (c < cols) v[j] = row[c];
   }
 }
 template <bool VEC, class T>
