@@ -326,9 +326,10 @@ int lbrr_op_feed_forward_noalloc(const uint16_t* h16, const uint16_t* w1_16, con
 
 /* ---------------------------------------------------------------------------
  * Matrix products in 8-bit floating point.  They have no counterpart in the
- * reference, whose products are fp16; they give the trunk's products (QKV,
- * out-projection, feed-forward) a form with half the operand bytes and twice
- * the tensor rate.
+ * reference, whose products are fp16; they give the trunk's products (the QKV
+ * projection without RoPE, out-projection, feed-forward) a form with half the
+ * operand bytes, for few rows and for weights held in 8 bits.  The fp16 entry
+ * points above are faster for a full chunk's feed-forward.
  *
  * An 8-bit matrix is two arrays.  `q`: e4m3 codes, rows `ldq` bytes apart.
  * `scales`: one fp32 scale per block of 128 columns and 1 row (activations) or
@@ -374,7 +375,9 @@ int lbrr_op_add_norm_quant8(const void* x, int32_t x_type, int64_t ldx, const vo
 
 /* out[m][n] = A W^T + bias[n] + resid[m][n]: A [m][k] scaled by 1 x 128, W [n][k]
  * scaled by 128 x 128 (the torch Linear layout), fp32 sums, one rounding to
- * out_type.  a and w must start on 16-byte boundaries with lda and ldw
+ * out_type.  The product of a block's two scales is formed in fp32 too: one below
+ * its normal range (values near 1e-19 on both sides) loses bits or vanishes, one
+ * above it is infinite.  a and w must start on 16-byte boundaries with lda and ldw
  * multiples of 16; any m, n, k >= 1.  bias (fp32) and resid (out_type) may be
  * NULL; resid may be out itself (same pointer and distance). */
 int lbrr_op_gemm8(const uint8_t* a, int64_t lda, const float* a_scales, int64_t ldas, const uint8_t* w, int64_t ldw,

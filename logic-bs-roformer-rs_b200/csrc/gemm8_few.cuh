@@ -19,9 +19,9 @@
 // that it does not need, and the code is kept short, because its first execution
 // waits for instruction fetches.
 //
-// Measured: 1 x 4096 x 4096 5.8 us (2.9 TB/s of weights; the tiled kernel 16.8),
-// 1 x 32768 x 4096 23 us (5.8 TB/s), 62 x 1536 x 256 5.1 us and 62 x 1024 x 256
-// with GELU to 8 bits 5.5 us, of which a launch is about 2.5.  Remote loads of
+// Measured: 1 x 4096 x 4096 6.0 us (2.8 TB/s of weights; the tiled kernel 16.8),
+// 1 x 32768 x 4096 23 us (5.8 TB/s), 62 x 1536 x 256 5.2 us and 62 x 1024 x 256
+// with GELU to 8 bits 6.0 us, of which a launch is about 2.5.  Remote loads of
 // the totals by the rows' warps took 1 us longer at 62 rows, remote stores 5 us.
 #pragma once
 #include "cp_async.cuh"

@@ -4,8 +4,8 @@
 // value is read once, held in registers while its block's or row's statistics
 // form, and written once), so HBM bounds them where there are rows enough to
 // fill the GPU.  What made the difference was having the next rows' loads in
-// flight while a block is worked on (71362 x 512 fp16 28 -> 20 us, 5.5 TB/s;
-// norm 4099 x 5000 bf16 46 -> 30 us, 4.8 TB/s) and few instructions per value (a
+// flight while a block is worked on (71362 x 512 fp16 28 -> 20 us, 5.4 TB/s;
+// norm 4099 x 5000 bf16 46 -> 29 us, 5.0 TB/s) and few instructions per value (a
 // division per block, sixteen compares per eight values and a reduction per
 // block cost 15-25 %).  Norm of 71362 x 256 (fp16 branch, fp32 stream): 33 us,
 // 6.0 TB/s.
@@ -91,9 +91,9 @@ __global__ void __launch_bounds__(kWarps8 * 32, kBlocksPerSm8<T, VEC, NARROW>)
 }
 
 // Blocks of 128 x 128: 32 values per thread.  16-bit inputs: two CTAs per SM
-// walk the blocks with the next one's loads in flight (71362 x 512: 33 -> 22 us);
+// walk the blocks with the next one's loads in flight (71362 x 512: 33 -> 21 us);
 // 32-bit inputs and unaligned rows leave no registers for that, so each block has
-// its own CTA (8192 x 8192 fp32: 51 us, 61 with the loop; 9402 x 1227 bf16: 10.6
+// its own CTA (8192 x 8192 fp32: 51 us, 61 with the loop; 9402 x 1227 bf16: 11
 // and 16.6).  `blocks_x`: blocks side by side.
 constexpr int kTileThreads8 = 512;
 template <class T, bool VEC>
