@@ -61,7 +61,7 @@ __device__ __forceinline__ Scale8 scale8(uint32_t top) {
 
 // Division of a block's values by its scale: v hi + v lo in one FMA after a
 // product, hi + lo = 1 / s to 2^-44 (a sum of two fp32 numbers, Dekker, Numer.
-// Math. 18, 1971; lo is hi's Newton correction), so the result is v / s rounded
+// Math. 18, 1971; lo is hi's correction of second order), so the result is v / s rounded
 // once, the fp32 quotient but for quotients that close to the middle between two
 // fp32 numbers.  hi is taken a little low: lo is then positive, and a zero keeps
 // its sign.  lo would leave the normal range beside a huge s, so those blocks are
@@ -78,7 +78,8 @@ __device__ __forceinline__ Quotient8 quotient8(Scale8 by) {
   const float s = huge ? by.s * kHugeDown8 : by.s;
   Quotient8 r;
   r.hi = (huge ? by.inv * (1.0f / kHugeDown8) : by.inv) * (1.0f - 0x1p-22f);
-  r.lo = fmaf(-s, r.hi, 1.0f) * r.hi;
+  const float e = fmaf(-s, r.hi, 1.0f);  // up to 2^-21: 1 / s = hi (1 + e + e^2 + ..)
+  r.lo = fmaf(e, e, e) * r.hi;
   return r;
 }
 
